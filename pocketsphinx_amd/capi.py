@@ -68,7 +68,8 @@ def build_library(force=False, extra_flags=(), lib_path=None, build_dir=None):
     flags = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off",
              # packed fp32 (v_pk_*) runs at half rate on gfx950 and the SLP pass
              # doubles register pressure here: keep the distance chain scalar
-             "-fno-slp-vectorize", "-Wno-unused-value", "-Wno-unused-result", "-fPIC", "-I" + os.path.join(ROOT, "include")] + list(extra_flags)
+             # -packed-fp32-ops: no v_pk_add / mul / fma_f32 at all (the host pass says it does not know the feature: harmless)
+             "-fno-slp-vectorize", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wno-unused-value", "-Wno-unused-result", "-fPIC", "-I" + os.path.join(ROOT, "include")] + list(extra_flags)
     bdir = build_dir or os.path.join(PKG_DIR, "_build")
     os.makedirs(bdir, exist_ok=True)
     newest_hdr = max(os.path.getmtime(h) for h in hdrs)
