@@ -41,7 +41,7 @@ extern "C" {
  * minor counts the additions) and asks psgpu_capabilities() for what the loaded library serves before it relies on an
  * optional part -- the reference has the same two-step in its own plugin loading: a name in the vtable, then the calls
  * (acmod.h:98-116). */
-#define PSGPU_ABI_VERSION  ((1 << 16) | 6)
+#define PSGPU_ABI_VERSION  ((1 << 16) | 7)
 #define PSGPU_CAP_PTM                 (1ull << 0)   /* psgpu_ptm_* (ptm_mgau.c) */
 #define PSGPU_CAP_SEMI                (1ull << 1)   /* psgpu_semi_* (s2_semi_mgau.c) */
 #define PSGPU_CAP_MS                  (1ull << 2)   /* psgpu_ms_* (ms_mgau.c, ms_gauden.c, ms_senone.c) */
@@ -57,6 +57,7 @@ extern "C" {
 #define PSGPU_CAP_FWDTREE_SPLIT       (1ull << 12)  /* one utterance's tree search on several workgroups */
 #define PSGPU_CAP_LM_SETS             (1ull << 14)  /* class words in a trie model; psgpu_lm_create_interp: an interpolated model set */
 #define PSGPU_CAP_FEAT_TYPES          (1ull << 13)  /* psgpu_feat_create: every feature type of feat_init, -lda, -svspec, varnorm, agc max */
+#define PSGPU_CAP_NET                 (1ull << 15)  /* psgpu_proj_*, psgpu_group_norm_*, psgpu_senone_scores_dev: layers of an acoustic network */
 int32_t psgpu_abi_version(void);
 uint64_t psgpu_capabilities(void);
 const char *psgpu_version(void);
@@ -1166,6 +1167,68 @@ int psgpu_decode_second_pass(psgpu_decode_t *d, psgpu_fwdflat_t *flat, void *str
  * senscr is the frame's n_sen int16 scores.  Synchronous. */
 int psgpu_hmm_vit_eval(psgpu_hmm_ctx_t *c, psgpu_hmm_rec_t *recs, int32_t n,
                        const int16_t *senscr, int32_t *best);
+
+/* ---- layers of an acoustic network beside the decoder (PSGPU_CAP_NET) ---------------------------------------------------------
+ * The reference decodes from senone scores made elsewhere (ps_decode_senscr, pocketsphinx.c:1199-1218; pocketsphinx_batch -senin;
+ * acmod_set_insenfh), as the searches here do (psgpu_fwdtree_search_dev's senscr_dev).  These make such scores on the device: a
+ * projection that all utterances share with a low-rank adapter per utterance, group norm with an activation, and the senone scores of
+ * a network's outputs.  Rows are frames of utterances back to back, utt_off_dev [n_utt + 1] as everywhere in this header; rows in
+ * front of the first utterance or behind the last one (a padded batch) are left as they are.  total_frames = the rows of the buffers;
+ * offsets that name rows outside them name no rows.  Row strides are in elements.  Element types: PSGPU_DT_*; sums run in 32 bits or
+ * more.  Everything is asynchronous on `stream`, allocates nothing, touches the caller's buffers alone and can be captured into a
+ * graph; a captured call's workspace belongs to that graph as long as it is replayed, so calls that may run at the same time need a
+ * workspace each. */
+#define PSGPU_DT_F32   0
+#define PSGPU_DT_F16   1
+#define PSGPU_DT_BF16  2
+#define PSGPU_ACT_NONE 0
+#define PSGPU_ACT_RELU 1
+#define PSGPU_ACT_SILU 2          /* v / (1 + exp(-v)) */
+#define PSGPU_ACT_GELU 3          /* v (1 + erf(v / sqrt 2)) / 2 */
+#define PSGPU_PROJ_MAX_RANK 128
+
+/* y[t] = bias + W x[t] + scale_a B_a (A_a x[t]), a the adapter of row t's utterance: a shared transform (what -lda is for the features,
+ * lda.c:139-159) with each speaker's own correction (what -mllr is for one decoder's means).  The object lives on the device that is
+ * current at its creation, where its calls must be made.
+ *  weight        [d_out][d_in] of `dtype`, host; bias [d_out] float, host, or NULL
+ *  max_adapters  slots for adapters, max_rank (1..PSGPU_PROJ_MAX_RANK) the largest rank one may have
+ * psgpu_proj_set_adapter: a [rank][d_in] and b [d_out][rank] of `dtype`, host, into a slot (replacing what it holds); rank 0 (a, b NULL)
+ * empties it.  It waits for the device, so that no call sees half an adapter; a graph replayed afterwards uses the new one.
+ * psgpu_proj_run_dev: x_dev [total_frames][x_stride], y_dev [total_frames][y_stride] of y_dtype (`dtype` or PSGPU_DT_F32), not
+ * overlapping.  utt_off_dev NULL: every row, no adapters (adapter_dev NULL).  adapter_dev [n_utt] slots; any value that names no
+ * loaded adapter (-1 by convention) means none.  work_dev: psgpu_proj_work_bytes(p, total_frames) bytes, 16-byte aligned, not needed
+ * without utt_off_dev. */
+typedef struct psgpu_proj_s psgpu_proj_t;
+int psgpu_proj_create(psgpu_proj_t **out, int32_t dtype, int32_t d_in, int32_t d_out, const void *weight, const float *bias,
+                      int32_t max_adapters, int32_t max_rank);
+void psgpu_proj_free(psgpu_proj_t *p);
+int psgpu_proj_set_adapter(psgpu_proj_t *p, int32_t slot, int32_t rank, const void *a, const void *b, float scale);
+int32_t psgpu_proj_d_in(const psgpu_proj_t *p);
+int32_t psgpu_proj_d_out(const psgpu_proj_t *p);
+size_t psgpu_proj_work_bytes(const psgpu_proj_t *p, int32_t total_frames);
+int psgpu_proj_run_dev(psgpu_proj_t *p, const void *x_dev, int64_t x_stride, const int32_t *utt_off_dev, const int32_t *adapter_dev,
+                       int32_t n_utt, int32_t total_frames, void *y_dev, int64_t y_stride, int32_t y_dtype, void *work_dev,
+                       size_t work_bytes, void *stream);
+
+/* y[t][c] = act((x[t][c] - m) / sqrt(v + eps) * weight[c] + bias[c]), m and v the mean and the biased variance of an utterance's frames x
+ * the channels of c's group (n_chan / n_groups neighbouring channels): cmn() with -varnorm (cmn.c:166-233) per group, with a learned
+ * scale.  weight_dev / bias_dev [n_chan] float or NULL (1 / 0).  y_dev has x_dev's type; it may be x_dev with the same stride, and may
+ * not overlap it otherwise.  An utterance of a live stream's step is normalised over that step's frames.  At most 65535 utterances.
+ * work_dev: psgpu_group_norm_work_bytes bytes, 16-byte aligned (may be NULL when that is 0). */
+size_t psgpu_group_norm_work_bytes(int32_t n_utt, int32_t total_frames, int32_t n_groups);
+int psgpu_group_norm_dev(int32_t dtype, const void *x_dev, int64_t x_stride, const int32_t *utt_off_dev, int32_t n_utt,
+                         int32_t total_frames, int32_t n_chan, int32_t n_groups, const float *weight_dev, const float *bias_dev,
+                         float eps, int32_t act, void *y_dev, int64_t y_stride, void *work_dev, size_t work_bytes, void *stream);
+
+/* A network's outputs z (before the softmax) as a search's scores: with l = z - log_prior (log_prior_dev [n_sen] float or NULL),
+ *   senscr[t][s] = min(32767, floor((max l[t] - l[t][s]) * scale / (1024 ln(logbase)) + 1/2)),
+ * the scaled log-likelihood over the frame's best in the units of the reference's scores (-logbase, SENSCR_SHIFT), lower is better;
+ * taken in 64 bits.  The rows are normalised over all senones (as with -compallsen) and serve as un-normalised rows alike.  -inf, a
+ * masked senone: 32767; a NaN counts as -inf here.  best_dev [total_frames] float or NULL: max l[t] - log sum exp z[t], the best
+ * senone's log-likelihood (-inf where every senone is masked, NaN where an output is). */
+int psgpu_senone_scores_dev(int32_t dtype, const void *logits_dev, int64_t logits_stride, int32_t total_frames, int32_t n_sen,
+                            const float *log_prior_dev, float scale, double logbase, int16_t *senscr_dev, int64_t senscr_stride,
+                            float *best_dev, void *stream);
 
 #ifdef __cplusplus
 }

@@ -20,5 +20,6 @@ from .search import FwdtreeSearch, backtrace  # noqa: F401
 from .lm import NGramTrieLM  # noqa: F401
 from .flat import FwdflatSearch  # noqa: F401
 from .decode import DecodePipeline  # noqa: F401
+from .net import AdaptedProjection, group_norm, senone_scores  # noqa: F401
 
-__all__ = ["PsgpuError", "lib", "build_library", "LIB_PATH", "PtmModel", "PtmMgau", "PtmState", "HmmContext", "HMM_REC", "SemiMgau", "MsMgau", "dynfeat_1s_c_d_dd", "FrontEnd", "FwdtreeSearch", "backtrace", "NGramTrieLM", "FwdflatSearch", "DecodePipeline"]
+__all__ = ["PsgpuError", "lib", "build_library", "LIB_PATH", "PtmModel", "PtmMgau", "PtmState", "HmmContext", "HMM_REC", "SemiMgau", "MsMgau", "dynfeat_1s_c_d_dd", "FrontEnd", "FwdtreeSearch", "backtrace", "NGramTrieLM", "FwdflatSearch", "DecodePipeline", "AdaptedProjection", "group_norm", "senone_scores"]

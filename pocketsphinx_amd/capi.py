@@ -8,7 +8,8 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG_DIR)
 LIB_PATH = os.environ.get("PSGPU_LIB_PATH") or os.path.join(PKG_DIR, "libpsgpu.so")     # (PSGPU_LIB_PATH: a measuring build, tools/build_prof_lib.py)
 CSRC = os.path.join(PKG_DIR, "csrc")
-SOURCES = ["psgpu_core.hip", "psgpu_ptm.hip", "psgpu_ptm_frame.hip", "psgpu_hmm.hip", "psgpu_semi.hip", "psgpu_ms.hip", "psgpu_feat.hip", "psgpu_fe.hip", "psgpu_search.hip", "psgpu_lm.hip", "psgpu_flat.hip", "psgpu_decode.hip"]
+SOURCES = ["psgpu_core.hip", "psgpu_ptm.hip", "psgpu_ptm_frame.hip", "psgpu_hmm.hip", "psgpu_semi.hip", "psgpu_ms.hip", "psgpu_feat.hip", "psgpu_fe.hip", "psgpu_search.hip", "psgpu_lm.hip", "psgpu_flat.hip", "psgpu_decode.hip",
+           "psgpu_proj.hip", "psgpu_gnorm.hip", "psgpu_netscr.hip"]
 
 # per-source flags (after the common ones).  The tree search is ONE kernel of ~9,000 instructions whose frame loop is a chain of
 # dependent steps: its speed follows the number of scalar values the compiler keeps alive (what does not fit the scalar registers is
@@ -44,6 +45,8 @@ SYMBOLS = [
     "psgpu_decode_view", "psgpu_decode_fetch_hyps", "psgpu_decode_fetch_tables", "psgpu_decode_fetch_tables_range", "psgpu_decode_stage_timing", "psgpu_decode_last_stage_ms", "psgpu_decode_search_after", "psgpu_decode_wait_scored", "psgpu_stream_create_dedicated", "psgpu_stream_destroy", "psgpu_fwdtree_hyp_out", "psgpu_decode_table_capacity", "psgpu_decode_second_pass", "psgpu_decode_tables_grown", "psgpu_decode_search_lag", "psgpu_fwdtree_search_lag", "psgpu_fwdtree_search_resume", "psgpu_fwdtree_search_streams", "psgpu_fwdtree_search_restart", "psgpu_phone_loop_carry_restart", "psgpu_decode_live_begin", "psgpu_decode_live_restart", "psgpu_decode_streams_begin", "psgpu_decode_streams_step", "psgpu_decode_streams_restart", "psgpu_decode_streams_next_utt", "psgpu_decode_live_step", "psgpu_decode_live_frames_searched", "psgpu_phone_loop_run_carry_dev", "psgpu_phone_loop_carry_words", "psgpu_decode_set_scorer", "psgpu_decode_compallsen", "psgpu_ms_score_batch_raw_dev", "psgpu_ms_batch_needs_lists", "psgpu_ms_list_entries_per_frame", "psgpu_semi_n_sen", "psgpu_semi_score_batch_carry_dev", "psgpu_semi_n_feat", "psgpu_semi_topn", "psgpu_semi_veclen",
     "psgpu_fwdflat_create", "psgpu_fwdflat_free", "psgpu_fwdflat_set_lm", "psgpu_fwdflat_search_dev", "psgpu_fwdflat_search_feats_dev", "psgpu_fwdflat_search_feats_lists_dev", "psgpu_ptm_batch_open_flags", "psgpu_ptm_model_view",
     "psgpu_lm_create", "psgpu_lm_create_interp", "psgpu_lm_free", "psgpu_lm_tg_score_dev",
+    "psgpu_proj_create", "psgpu_proj_free", "psgpu_proj_set_adapter", "psgpu_proj_d_in", "psgpu_proj_d_out", "psgpu_proj_work_bytes", "psgpu_proj_run_dev",
+    "psgpu_group_norm_work_bytes", "psgpu_group_norm_dev", "psgpu_senone_scores_dev",
 ]
 
 
@@ -160,6 +163,20 @@ def lib():
     L.psgpu_hmm_n_emit_state.argtypes = [vp]
     L.psgpu_hmm_vit_eval_dev.argtypes = [vp, vp, vp, i32, vp, vp, i32, vp, vp]
     L.psgpu_hmm_vit_eval.argtypes = [vp, vp, i32, vp, C.POINTER(i32)]
+    i64, sz, f32 = C.c_int64, C.c_size_t, C.c_float
+    L.psgpu_proj_create.argtypes = [C.POINTER(vp), i32, i32, i32, vp, vp, i32, i32]
+    L.psgpu_proj_free.argtypes = [vp]
+    L.psgpu_proj_free.restype = None
+    L.psgpu_proj_set_adapter.argtypes = [vp, i32, i32, vp, vp, f32]
+    L.psgpu_proj_d_in.argtypes = [vp]
+    L.psgpu_proj_d_out.argtypes = [vp]
+    L.psgpu_proj_work_bytes.argtypes = [vp, i32]
+    L.psgpu_proj_work_bytes.restype = sz
+    L.psgpu_proj_run_dev.argtypes = [vp, vp, i64, vp, vp, i32, i32, vp, i64, i32, vp, sz, vp]
+    L.psgpu_group_norm_work_bytes.argtypes = [i32, i32, i32]
+    L.psgpu_group_norm_work_bytes.restype = sz
+    L.psgpu_group_norm_dev.argtypes = [i32, vp, i64, vp, i32, i32, i32, i32, vp, vp, f32, i32, vp, i64, vp, sz, vp]
+    L.psgpu_senone_scores_dev.argtypes = [i32, vp, i64, i32, i32, vp, f32, C.c_double, vp, i64, vp, vp]
     L.psgpu_ptm_kernel_timing.argtypes = [vp, i32]
     L.psgpu_ptm_last_kernel_ms.argtypes = [vp, C.POINTER(C.c_float)]
     L.psgpu_event_create.argtypes = [C.POINTER(vp)]
