@@ -1227,7 +1227,7 @@ int psgpu_group_norm_dev(int32_t dtype, const void *x_dev, int64_t x_stride, con
  * masked senone: 32767; a NaN counts as -inf here.  best_dev [total_frames] float or NULL: max l[t] - log sum exp z[t], the best
  * senone's log-likelihood (-inf where every senone is masked, NaN where an output is). */
 int psgpu_senone_scores_dev(int32_t dtype, const void *logits_dev, int64_t logits_stride, int32_t total_frames, int32_t n_sen,
-                            const float *log_prior_dev, float scale, double logbase, int16_t *senscr_dev, int64_t senscr_stride,
+                            const float *log_prior_dev, double scale, double logbase, int16_t *senscr_dev, int64_t senscr_stride,
                             float *best_dev, void *stream);
 
 #ifdef __cplusplus

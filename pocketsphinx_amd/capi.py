@@ -176,7 +176,7 @@ def lib():
     L.psgpu_group_norm_work_bytes.argtypes = [i32, i32, i32]
     L.psgpu_group_norm_work_bytes.restype = sz
     L.psgpu_group_norm_dev.argtypes = [i32, vp, i64, vp, i32, i32, i32, i32, vp, vp, f32, i32, vp, i64, vp, sz, vp]
-    L.psgpu_senone_scores_dev.argtypes = [i32, vp, i64, i32, i32, vp, f32, C.c_double, vp, i64, vp, vp]
+    L.psgpu_senone_scores_dev.argtypes = [i32, vp, i64, i32, i32, vp, C.c_double, C.c_double, vp, i64, vp, vp]
     L.psgpu_ptm_kernel_timing.argtypes = [vp, i32]
     L.psgpu_ptm_last_kernel_ms.argtypes = [vp, C.POINTER(C.c_float)]
     L.psgpu_event_create.argtypes = [C.POINTER(vp)]

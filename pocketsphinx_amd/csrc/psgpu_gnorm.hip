@@ -80,7 +80,7 @@ extern "C" int psgpu_group_norm_dev(int32_t dtype, const void *x_dev, int64_t x_
     PSGPU_REQUIRE(work_bytes >= psgpu_group_norm_work_bytes(n_utt, total_frames, n_groups) && (work_dev || !psgpu_group_norm_work_bytes(n_utt, total_frames, n_groups)),
                   "psgpu_group_norm_dev: %zu bytes of workspace, psgpu_group_norm_work_bytes asks for %zu", work_bytes,
                   psgpu_group_norm_work_bytes(n_utt, total_frames, n_groups));
-    const int rc = psgpu_check_device();
+    const int rc = net_check_device(nullptr);
     if (rc != PSGPU_OK) return rc;
     const dim3 grid((uint32_t)n_groups, (uint32_t)n_utt);
     const hipStream_t st = (hipStream_t)stream;

@@ -37,8 +37,48 @@ __device__ __forceinline__ int net_utt_of_row(const int32_t *off, int n_utt, int
     return lo < n_utt && off[lo] <= row ? lo : -1;
 }
 
+// ---- matrix instructions ------------------------------------------------------------------------------------------------------------
+// Products of 16 x 16 from 16 bytes a lane: lane l of the first operand holds row l & 15, of the second column l & 15, elements
+// (l >> 4) * E .. + E - 1 of the reduced axis (E = 16 bytes of T; one instruction of 4 E elements for halves, four of 4 for floats, which
+// take element j of every lane's chunk -- the same order on both sides, so the sum is the same set of products).  Lane l holds of the
+// result column l & 15, rows (l >> 4) * 4 .. + 3.
+typedef float net_f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 net_f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 net_bf16x8 __attribute__((ext_vector_type(8)));
+template <typename T> struct net_frag;
+template <> struct net_frag<float> { typedef net_f32x4 type; };
+template <> struct net_frag<psg_half> { typedef net_f16x8 type; };
+template <> struct net_frag<psg_bf16> { typedef net_bf16x8 type; };
+
+__device__ __forceinline__ net_f32x4 net_mfma(net_f32x4 a, net_f32x4 b, net_f32x4 c)
+{
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+}
+__device__ __forceinline__ net_f32x4 net_mfma(net_f16x8 a, net_f16x8 b, net_f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ net_f32x4 net_mfma(net_bf16x8 a, net_bf16x8 b, net_f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+// E elements of a row from k on, zeros from d_in on; any alignment
+template <typename T>
+__device__ __forceinline__ typename net_frag<T>::type net_load_chunk(const T *row, int k, int d_in)
+{
+    constexpr int E = 16 / sizeof(T);
+    net_pack<T, E> v;
+    if (k + E <= d_in) v = *(const net_pack<T, E> *)(row + k);
+    else {
+        v = {};
+        for (int e = 0; e < E; ++e)
+            if (k + e < d_in) v.v[e] = row[k + e];
+    }
+    return __builtin_bit_cast(typename net_frag<T>::type, v);
+}
+
 static inline size_t net_dtype_size(int32_t dtype) { return dtype == PSGPU_DT_F32 ? 4 : 2; }
 static inline bool net_dtype_ok(int32_t dtype) { return dtype == PSGPU_DT_F32 || dtype == PSGPU_DT_F16 || dtype == PSGPU_DT_BF16; }
+// PSGPU_OK iff a gfx950 device is current, which one; asks the runtime about a device's kind once
+int net_check_device(int *device);
+
 // bytes that rows of `width` elements at `stride` cover
 static inline size_t net_span(int64_t rows, int64_t stride, int64_t width, size_t es) { return rows ? (size_t)((rows - 1) * stride + width) * es : 0; }
 static inline bool net_disjoint(const void *a, size_t na, const void *b, size_t nb)

@@ -9,6 +9,7 @@
 // ptm_mgau_senone_eval's normalisation does (ptm_mgau.c:398-400); it stays in best[] alone.  Differences are taken in 64 bits: a score
 // next to a rounding border is decided by their last bits, and the reference's scores are whole numbers that a search compares.
 #include "psgpu_net_dev.h"
+#include <atomic>
 #include <cmath>
 
 constexpr int kScrThreads = 256;
@@ -61,23 +62,39 @@ void netscr_row_kernel(const T *__restrict__ z, int64_t z_stride, int32_t n_sen,
     }
 }
 
+// hipGetDeviceProperties costs more than a launch: its answer for a device is kept
+int net_check_device(int *device)
+{
+    static std::atomic<uint8_t> good[64];
+    int d = -1;
+    if (hipGetDevice(&d) == hipSuccess && d >= 0 && d < 64 && good[d].load(std::memory_order_relaxed)) {
+        if (device) *device = d;
+        return PSGPU_OK;
+    }
+    const int rc = psgpu_check_device();
+    if (rc != PSGPU_OK) return rc;
+    if (d >= 0 && d < 64) good[d].store(1, std::memory_order_relaxed);
+    if (device) *device = d;
+    return PSGPU_OK;
+}
+
 extern "C" int psgpu_senone_scores_dev(int32_t dtype, const void *logits_dev, int64_t logits_stride, int32_t total_frames, int32_t n_sen,
-                                       const float *log_prior_dev, float scale, double logbase, int16_t *senscr_dev,
+                                       const float *log_prior_dev, double scale, double logbase, int16_t *senscr_dev,
                                        int64_t senscr_stride, float *best_dev, void *stream)
 {
     psgpu_clear_error();
     PSGPU_REQUIRE(net_dtype_ok(dtype), "psgpu_senone_scores_dev: dtype %d", dtype);
     PSGPU_REQUIRE(total_frames >= 0 && n_sen >= 1, "psgpu_senone_scores_dev: %d frames of %d senones", total_frames, n_sen);
     PSGPU_REQUIRE(logits_stride >= n_sen && senscr_stride >= n_sen, "psgpu_senone_scores_dev: a row stride is below %d", n_sen);
-    PSGPU_REQUIRE(std::isfinite(scale) && scale > 0.0f, "psgpu_senone_scores_dev: scale %g", (double)scale);
+    PSGPU_REQUIRE(std::isfinite(scale) && scale > 0.0, "psgpu_senone_scores_dev: scale %g", scale);
     PSGPU_REQUIRE(std::isfinite(logbase) && logbase > 1.0, "psgpu_senone_scores_dev: logbase %g", logbase);
     if (total_frames == 0) return PSGPU_OK;
     PSGPU_REQUIRE(logits_dev && senscr_dev, "psgpu_senone_scores_dev: NULL device buffer");
     PSGPU_REQUIRE(net_disjoint(logits_dev, net_span(total_frames, logits_stride, n_sen, net_dtype_size(dtype)), senscr_dev,
                                net_span(total_frames, senscr_stride, n_sen, 2)), "psgpu_senone_scores_dev: the scores overlap the logits");
-    const int rc = psgpu_check_device();
+    const int rc = net_check_device(nullptr);
     if (rc != PSGPU_OK) return rc;
-    const double unit = (double)scale / (std::log(logbase) * (double)(1 << kSenscrShift));
+    const double unit = scale / (std::log(logbase) * (double)(1 << kSenscrShift));
     const dim3 grid((uint32_t)total_frames);
     const hipStream_t st = (hipStream_t)stream;
     if (dtype == PSGPU_DT_F32)

@@ -96,7 +96,7 @@ def senones(z, prior, scale, logbase):
     l = zz - p
     l = np.where(np.isnan(l), -np.inf, l)
     top = l.max(axis=1)
-    unit = float(np.float32(scale)) / (math.log(logbase) * 1024)
+    unit = scale / (math.log(logbase) * 1024)
     with np.errstate(invalid="ignore", over="ignore"):
         d = np.floor((top[:, None] - l) * unit + 0.5)
     d = np.where(l == -np.inf, 32767, np.where(l == top[:, None], 0, d))
