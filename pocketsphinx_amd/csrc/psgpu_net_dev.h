@@ -14,27 +14,46 @@ __device__ __forceinline__ float net_f32(psg_bf16 v) { return __uint_as_float((u
 template <typename T> __device__ __forceinline__ T net_cast(float v);
 template <> __device__ __forceinline__ float net_cast<float>(float v) { return v; }
 template <> __device__ __forceinline__ psg_half net_cast<psg_half>(float v) { return (psg_half)v; }
-template <> __device__ __forceinline__ psg_bf16 net_cast<psg_bf16>(float v)
-{
-    const uint32_t u = __float_as_uint(v);
-    psg_bf16 r;
-    r.bits = (u & 0x7fffffffu) > 0x7f800000u ? (uint16_t)((u >> 16) | 0x40) : (uint16_t)((u + 0x7fffu + ((u >> 16) & 1)) >> 16);
-    return r;
-}
+template <> __device__ __forceinline__ psg_bf16 net_cast<psg_bf16>(float v) { return __builtin_bit_cast(psg_bf16, (__bf16)v); }
 
 // N consecutive elements that need no alignment beyond their own: the hardware serves wide loads and stores at any element address
 template <typename T, int N> struct __attribute__((packed, aligned(sizeof(T)))) net_pack { T v[N]; };
 
-// The utterance of a packed row: the u with off[u] <= row < off[u + 1], or -1 (in front of the first, behind the last).  Empty
-// utterances are stepped over.  Offsets that do not ascend give some u or -1, never an access outside off[0 .. n_utt].
-__device__ __forceinline__ int net_utt_of_row(const int32_t *off, int n_utt, int row)
+// The utterance of each of 64 packed rows, row0 + lane: the u with off[u] <= row < off[u + 1], or -1 (in front of the first, behind
+// the last).  Empty utterances are stepped over.  Offsets that do not ascend give some u or -1, never an access outside
+// off[0 .. n_utt].  All lanes of the wavefront call it.  64 offsets a step for the first row (two dependent loads for 4096 utterances;
+// a binary search would wait for 12), then the 64 offsets behind it for the rest.
+__device__ __forceinline__ int net_utt_of_rows(const int32_t *off, int n_utt, int row0)
 {
-    int lo = 0, hi = n_utt;                         // first u in [0, n_utt] with off[u + 1] > row
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (off[mid + 1] > row) hi = mid; else lo = mid + 1;
+    const int lane = (int)(threadIdx.x & 63), row = row0 + lane;
+    int lo = 0, hi = n_utt;                         // the first u in [lo, hi] with off[u + 1] > row0 (hi: none)
+    while (hi - lo > 64) {
+        const int step = (hi - lo + 63) >> 6, at = lo + lane * step;
+        const uint64_t above = __ballot(at >= hi || off[min(at, n_utt - 1) + 1] > row0);
+        const int f = above ? __builtin_ctzll(above) : 64;
+        hi = min(hi, lo + f * step);
+        lo = f ? min(hi, lo + (f - 1) * step + 1) : lo;
     }
-    return lo < n_utt && off[lo] <= row ? lo : -1;
+    // off[lo + 1 + lane], the last of them standing for all behind it
+    int v = lo + lane < n_utt ? off[lo + lane + 1] : 0x7fffffff;
+    const uint64_t above = __ballot(lo + lane >= hi || v > row0);
+    const int skip = above ? __builtin_ctzll(above) : 64;
+    lo += skip;
+    if (skip) v = lo + lane < n_utt ? off[lo + lane + 1] : 0x7fffffff;
+    int pos = 0;                                    // how many of the 64 offsets are not above this lane's row
+#pragma unroll
+    for (int s = 32; s; s >>= 1)
+        if (__shfl(v, pos + s - 1) <= row) pos += s;
+    int u = lo + pos;
+    if (pos == 63 && u < n_utt && off[u + 1] <= row) {      // more than 64 utterances end within these rows
+        int a = u + 1, b = n_utt;
+        while (a < b) {
+            const int mid = (a + b) >> 1;
+            if (off[mid + 1] > row) b = mid; else a = mid + 1;
+        }
+        u = a;
+    }
+    return u >= 0 && u < n_utt && off[u] <= row && off[u + 1] > row ? u : -1;
 }
 
 // ---- matrix instructions ------------------------------------------------------------------------------------------------------------

@@ -6,129 +6,558 @@
 // features, reference src/feat/lda.c:139-159, and -mllr for the means of one decoder's speaker, src/ps_mllr.c).  Products of the inputs'
 // type, sums in 32 bits, one rounding at the end.
 //
-// psgpu_proj_t keeps the weights and every loaded adapter on the device, laid out once:
-//   W  [Np][Kp], A per slot [Rp][Kp], B per slot [Np][Rp], zeros in the padding.
+// psgpu_proj_t keeps the weights and every loaded adapter on the device, laid out once in the order in which a wavefront's lanes hold
+// the first operand of a matrix instruction (a "fragment": 16 rows x 64 bytes of the reduced axis, 16 bytes a lane, 1 KB in a piece):
+//   W   [outs / 64][chunks][4][64 lanes][16 bytes]          a chunk: KC = 64 bytes of d_in
+//   A   [slot][chunks][ranks / 16][64 lanes][16 bytes]
+//   B   [slot][parts][outs / 64][ranks / KC][4][64 lanes][16 bytes]
+// zeros in the padding.  Fragment f of 64 outputs holds in row m the output (m / 4) * 16 + f * 4 + m % 4: the four fragments leave a
+// lane 16 neighbouring outputs of one frame, 128 bytes a frame in a store.
+//
+// The adapters' h is kept in 32 bits, for the half types as two bfloat16 parts (their sum is h to 2^-17) that go through the matrix
+// instructions as one more piece of the reduced axis, against B in bfloat16: float16's B is two parts (exact), of whose products the
+// smallest, 2^-16 of the term, is left out.  In float16 itself h could overflow.
 #include "psgpu_net_dev.h"
 #include <cmath>
 #include <cstring>
 #include <new>
-#include <vector>
+#include <type_traits>
 
 struct psgpu_proj_s {
     int device = 0;
     int32_t dtype = 0, d_in = 0, d_out = 0, max_adapters = 0, max_rank = 0;
     int32_t kp = 0, np = 0, rp = 0;                 // padded d_in, d_out, max_rank
+    size_t a_slot = 0, b_slot = 0;                  // bytes of a slot
     char *w = nullptr;
     float *bias = nullptr;                          // [np], zeros where there is none
     char *a = nullptr, *b = nullptr;                // [max_adapters] slots
     int32_t *rank = nullptr;                        // [max_adapters], 0: nothing loaded
     float *scale = nullptr;
+    char *raw = nullptr;                            // an adapter as it comes, before it is laid out
 };
 
 constexpr int kProjNoRow = -2;                      // rows of no utterance: left as they are
 
-// ---- one wavefront a row: which adapter it has, and h ------------------------------------------------------------------------------
-template <typename T>
-__global__ __launch_bounds__(64)
-void proj_shrink_kernel(const T *__restrict__ x, int64_t x_stride, int32_t d_in, int32_t kp, const T *__restrict__ a, int32_t rp,
-                        const int32_t *__restrict__ rank, const float *__restrict__ scale, int32_t max_adapters,
-                        const int32_t *__restrict__ utt_off, const int32_t *__restrict__ adapter, int32_t n_utt,
-                        int32_t *__restrict__ row_slot, float *__restrict__ h)
+template <typename T> struct proj_geo {
+    static constexpr int E = 16 / sizeof(T);        // elements a lane, elements a chunk
+    static constexpr int KC = 4 * E;
+    static constexpr int parts = sizeof(T) == 4 ? 1 : 2;    // of h
+    typedef typename net_frag<T>::type frag;
+};
+template <typename T> struct proj_b_type { typedef psg_bf16 type; static constexpr int parts = 1; };     // what B is kept in
+template <> struct proj_b_type<float> { typedef float type; static constexpr int parts = 1; };
+template <> struct proj_b_type<psg_half> { typedef psg_bf16 type; static constexpr int parts = 2; };
+
+__device__ __forceinline__ int proj_out_of(int f, int m) { return (m >> 2) * 16 + f * 4 + (m & 3); }
+
+// the two bfloat16 parts of a value (an infinity has a second part of 0)
+__device__ __forceinline__ void proj_split(float v, psg_bf16 &hi, psg_bf16 &lo)
 {
-    const size_t t = blockIdx.x;
-    const int lane = threadIdx.x;
-    const int u = net_utt_of_row(utt_off, n_utt, (int)t);
-    int slot = u < 0 ? kProjNoRow : (adapter ? adapter[u] : -1);
-    if (slot >= 0 && (slot >= max_adapters || rank[slot] == 0)) slot = -1;
-    if (slot < 0 && u >= 0) slot = -1;
-    if (lane == 0) row_slot[t] = slot;
-    if (slot < 0) return;
-    const T *ar = a + (size_t)slot * rp * kp;
-    const int r_n = rank[slot];
-    for (int r = 0; r < r_n; ++r) {
-        float s = 0.0f;
-        for (int k = lane; k < d_in; k += 64) s += net_f32(x[t * x_stride + k]) * net_f32(ar[(size_t)r * kp + k]);
-        for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
-        if (lane == 0) h[t * rp + r] = s * scale[slot];
+    hi = net_cast<psg_bf16>(v);
+    const float rest = v - net_f32(hi);
+    lo = net_cast<psg_bf16>(__builtin_isinf(net_f32(hi)) ? 0.0f : rest);
+}
+
+// ---- layouts, one 16-byte lane's share a work-item --------------------------------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(256)
+void proj_lay_w_kernel(const T *__restrict__ src, int32_t rows, int32_t cols, int32_t chunks, size_t n, T *__restrict__ dst)
+{
+    constexpr int E = proj_geo<T>::E, KC = proj_geo<T>::KC;
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    const int lane = i & 63, f = (i >> 6) & 3, c = (int)((i >> 8) % chunks);
+    const int o = (int)((i >> 8) / chunks) * 64 + proj_out_of(f, lane & 15), k = c * KC + (lane >> 4) * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) dst[i * E + e] = o < rows && k + e < cols ? src[(size_t)o * cols + k + e] : T{};
+}
+
+template <typename T>
+__global__ __launch_bounds__(256)
+void proj_lay_a_kernel(const T *__restrict__ src, int32_t rank, int32_t d_in, int32_t rank_frags, size_t n, T *__restrict__ dst)
+{
+    constexpr int E = proj_geo<T>::E, KC = proj_geo<T>::KC;
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    const int lane = i & 63, q = (int)((i >> 6) % rank_frags), c = (int)((i >> 6) / rank_frags);
+    const int r = q * 16 + (lane & 15), k = c * KC + (lane >> 4) * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) dst[i * E + e] = r < rank && k + e < d_in ? src[(size_t)r * d_in + k + e] : T{};
+}
+
+template <typename T>
+__global__ __launch_bounds__(256)
+void proj_lay_b_kernel(const T *__restrict__ src, int32_t d_out, int32_t rank, int32_t rank_chunks, size_t n, typename proj_b_type<T>::type *__restrict__ dst)
+{
+    constexpr int E = proj_geo<T>::E, KC = proj_geo<T>::KC;
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    const int lane = i & 63, f = (i >> 6) & 3, c = (int)((i >> 8) % rank_chunks);
+    const int o = (int)((i >> 8) / rank_chunks) * 64 + proj_out_of(f, lane & 15), r = c * KC + (lane >> 4) * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const T v = o < d_out && r + e < rank ? src[(size_t)o * rank + r + e] : T{};
+        if constexpr (proj_b_type<T>::parts == 2) {
+            psg_bf16 hi, lo;
+            proj_split(net_f32(v), hi, lo);
+            dst[i * E + e] = hi;
+            dst[(n + i) * E + e] = lo;
+        } else dst[i * E + e] = v;
     }
 }
 
-// ---- a 32 x 32 tile of y a workgroup ----------------------------------------------------------------------------------------------
-constexpr int kTile = 32;
-template <typename T, typename Y>
-__global__ __launch_bounds__(256)
-void proj_tile_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, int32_t d_in, int32_t kp, const T *__restrict__ w,
-                      const float *__restrict__ bias, int32_t d_out, const T *__restrict__ b, int32_t np, int32_t rp,
-                      const int32_t *__restrict__ rank, const int32_t *__restrict__ row_slot, const float *__restrict__ h,
-                      Y *__restrict__ y, int64_t y_stride)
+// which adapter a row has; the lane's row is row0 + lane, kProjNoRow beyond `total`
+__device__ __forceinline__ int proj_slot_of_rows(const int32_t *utt_off, const int32_t *adapter, int n_utt, const int32_t *rank, int max_adapters, int row0, int total)
 {
-    __shared__ float s_x[kTile][kTile + 1], s_w[kTile][kTile + 1];
-    const int r0 = blockIdx.y * kTile, o0 = blockIdx.x * kTile, tid = threadIdx.x;
-    const int o = tid & 31, r = tid >> 5;           // this work-item's column and its rows r, r + 8, r + 16, r + 24
-    float acc[4] = {0, 0, 0, 0};
-    for (int k0 = 0; k0 < d_in; k0 += kTile) {
-        for (int i = 0; i < 4; ++i) {
-            const int row = r0 + r + 8 * i;
-            s_x[r + 8 * i][o] = row < rows && k0 + o < d_in ? net_f32(x[(size_t)row * x_stride + k0 + o]) : 0.0f;
-            s_w[r + 8 * i][o] = net_f32(w[(size_t)(o0 + r + 8 * i) * kp + k0 + o]);
+    const int u = net_utt_of_rows(utt_off, n_utt, row0);
+    if (u < 0 || row0 + (int)(threadIdx.x & 63) >= total) return kProjNoRow;
+    const int slot = adapter ? adapter[u] : -1;
+    return slot >= 0 && slot < max_adapters && rank[slot] > 0 ? slot : -1;
+}
+
+// ---- h --------------------------------------------------------------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ void proj_store_h(net_f32x4 v, float scale, char *h, size_t t, int rp, int r)
+{
+    if constexpr (sizeof(T) == 4) {
+        net_f32x4 o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = v[i] * scale;
+        *(net_f32x4 *)((float *)h + t * rp + r) = o;
+    } else {
+        net_pack<psg_bf16, 4> hi, lo;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) proj_split(v[i] * scale, hi.v[i], lo.v[i]);
+        *(uint64_t *)((psg_bf16 *)h + t * 2 * rp + r) = __builtin_bit_cast(uint64_t, hi);
+        *(uint64_t *)((psg_bf16 *)h + t * 2 * rp + rp + r) = __builtin_bit_cast(uint64_t, lo);
+    }
+}
+
+// Many rows: 32 a wavefront, all of an adapter's ranks at once, x once from memory (that is what bounds it), A from the caches.
+template <typename T, int RF>
+__global__ __launch_bounds__(256)
+void proj_shrink_kernel(const T *__restrict__ x, int64_t x_stride, int32_t total, int32_t d_in, int32_t chunks, const char *__restrict__ a, size_t a_slot,
+                        int32_t rp, const int32_t *__restrict__ rank, const float *__restrict__ scale, int32_t max_adapters,
+                        const int32_t *__restrict__ utt_off, const int32_t *__restrict__ adapter, int32_t n_utt,
+                        int32_t *__restrict__ row_slot, char *__restrict__ h)
+{
+    constexpr int E = proj_geo<T>::E, KC = proj_geo<T>::KC;
+    typedef typename proj_geo<T>::frag frag;
+    const int lane = threadIdx.x & 63;
+    const int64_t row0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 32;
+    if (row0 >= total) return;
+    const int slot = proj_slot_of_rows(utt_off, adapter, n_utt, rank, max_adapters, (int)row0, total);
+    if (lane < 32 && row0 + lane < total) row_slot[row0 + lane] = slot;
+    if (!a) return;
+    const int rank_frags = rp / 16;
+    const T *x0 = x + min(row0 + (lane & 15), (int64_t)total - 1) * x_stride, *x1 = x + min(row0 + 16 + (lane & 15), (int64_t)total - 1) * x_stride;
+    uint64_t todo = __ballot(lane < 32 && slot >= 0);
+    while (todo) {
+        const int s = __shfl(slot, __builtin_ctzll(todo));
+        const uint64_t mine = __ballot(slot == s);
+        todo &= ~mine;
+        const frag *as = (const frag *)(a + s * a_slot) + lane;
+        net_f32x4 acc[2][RF] = {};
+#pragma unroll 2
+        for (int c = 0; c < chunks; ++c) {
+            const int k = c * KC + (lane >> 4) * E;
+            const frag f0 = net_load_chunk(x0, k, d_in), f1 = net_load_chunk(x1, k, d_in);
+#pragma unroll
+            for (int q = 0; q < RF; ++q) {
+                const frag w = as[(c * rank_frags + min(q, rank_frags - 1)) * 64];
+                acc[0][q] = net_mfma(w, f0, acc[0][q]);
+                acc[1][q] = net_mfma(w, f1, acc[1][q]);
+            }
+        }
+        const float sc = scale[s];
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+            if (mine >> (m * 16 + (lane & 15)) & 1)
+#pragma unroll
+                for (int q = 0; q < RF; ++q)
+                    if (q < rank_frags) proj_store_h<T>(acc[m][q], sc, h, (size_t)row0 + m * 16 + (lane & 15), rp, q * 16 + (lane >> 4) * 4);
+    }
+}
+
+// Few rows: `tile` (1 .. 16) a workgroup, whose four wavefronts share the reduced axis.
+template <typename T, int RF>
+__global__ __launch_bounds__(256)
+void proj_shrink_few_kernel(const T *__restrict__ x, int64_t x_stride, int32_t total, int32_t d_in, int32_t chunks, const char *__restrict__ a, size_t a_slot,
+                            int32_t rp, const int32_t *__restrict__ rank, const float *__restrict__ scale, int32_t max_adapters,
+                            const int32_t *__restrict__ utt_off, const int32_t *__restrict__ adapter, int32_t n_utt, int32_t tile,
+                            int32_t *__restrict__ row_slot, char *__restrict__ h)
+{
+    constexpr int E = proj_geo<T>::E, KC = proj_geo<T>::KC;
+    typedef typename proj_geo<T>::frag frag;
+    __shared__ net_f32x4 s_part[4][RF][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15;
+    const int64_t row0 = (int64_t)blockIdx.x * tile;
+    int slot = proj_slot_of_rows(utt_off, adapter, n_utt, rank, max_adapters, (int)row0, total);
+    if (lane >= tile) slot = kProjNoRow;
+    if (threadIdx.x < tile && row0 + lane < total) row_slot[row0 + lane] = slot;
+    if (!a) return;
+    const int rank_frags = rp / 16;
+    const T *xr = x + min(row0 + col, (int64_t)total - 1) * x_stride;
+    uint64_t todo = __ballot(slot >= 0);
+    while (todo) {                                  // (the same in all four)
+        const int s = __shfl(slot, __builtin_ctzll(todo));
+        const uint64_t mine = __ballot(slot == s);
+        todo &= ~mine;
+        const frag *as = (const frag *)(a + s * a_slot) + lane;
+        net_f32x4 acc[RF] = {};
+#pragma unroll 4
+        for (int c = wave; c < chunks; c += 4) {
+            frag f = {};
+            if (mine >> col & 1) f = net_load_chunk(xr, c * KC + (lane >> 4) * E, d_in);
+#pragma unroll
+            for (int q = 0; q < RF; ++q) acc[q] = net_mfma(as[(c * rank_frags + min(q, rank_frags - 1)) * 64], f, acc[q]);
+        }
+#pragma unroll
+        for (int q = 0; q < RF; ++q) s_part[wave][q][lane] = acc[q];
+        __syncthreads();
+        const float sc = scale[s];
+        for (int q = wave; q < rank_frags; q += 4) {
+            net_f32x4 v = s_part[0][q][lane];
+            for (int w = 1; w < 4; ++w) v += s_part[w][q][lane];
+            if (mine >> col & 1) proj_store_h<T>(v, sc, h, (size_t)row0 + col, rp, q * 16 + (lane >> 4) * 4);
         }
         __syncthreads();
-        for (int k = 0; k < kTile; ++k)
-            for (int i = 0; i < 4; ++i) acc[i] += s_x[r + 8 * i][k] * s_w[o][k];
-        __syncthreads();
     }
-    if (o0 + o >= d_out) return;
-    for (int i = 0; i < 4; ++i) {
-        const int row = r0 + r + 8 * i;
-        if (row >= rows) continue;
-        const int slot = row_slot ? row_slot[row] : -1;
+}
+
+// ---- the product in tiles -----------------------------------------------------------------------------------------------------------
+// acc of 16 frames (column lane & 15) += B_s h over the ranks of adapter s, for the frames whose slot it is
+template <typename T, int NF, int MF>
+__device__ __forceinline__ void proj_expand(net_f32x4 (&acc)[MF][NF], int m0, int m1, const int (&slot)[MF], int s, const char *b, size_t b_slot, size_t b_part, size_t b_group,
+                                            int chunks, int rp, const char *h, const int64_t (&t)[MF])
+{
+    constexpr int E = proj_geo<T>::E, KC = proj_geo<T>::KC;
+    typedef typename proj_b_type<T>::type B;
+    typedef typename net_frag<B>::type bfrag;
+    const int lane = threadIdx.x & 63;
+    const char *bs = b + s * b_slot + b_group;
+    for (int c = 0; c < chunks; ++c) {
+        bfrag w[NF], w2[NF];
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+            w[f] = ((const bfrag *)(bs + (size_t)(f >> 2) * rp * 64 * sizeof(B)))[(c * 4 + (f & 3)) * 64 + lane];
+            if constexpr (proj_b_type<T>::parts == 2) w2[f] = ((const bfrag *)(bs + b_part + (size_t)(f >> 2) * rp * 64 * sizeof(B)))[(c * 4 + (f & 3)) * 64 + lane];
+        }
+#pragma unroll
+        for (int m = 0; m < MF; ++m) {
+            if (m < m0 || m >= m1) continue;
+            bfrag hi = {}, lo = {};
+            if (slot[m] == s) {
+                const B *hr = (const B *)h + (size_t)t[m] * proj_geo<T>::parts * rp + c * KC + (lane >> 4) * E;
+                hi = *(const bfrag *)hr;
+                if constexpr (proj_geo<T>::parts == 2) lo = *(const bfrag *)(hr + rp);
+            }
+#pragma unroll
+            for (int f = 0; f < NF; ++f) {
+                acc[m][f] = net_mfma(w[f], hi, acc[m][f]);
+                if constexpr (proj_geo<T>::parts == 2) acc[m][f] = net_mfma(w[f], lo, acc[m][f]);
+                if constexpr (proj_b_type<T>::parts == 2) acc[m][f] = net_mfma(w2[f], hi, acc[m][f]);
+            }
+        }
+    }
+}
+
+typedef const __attribute__((address_space(1))) uint32_t *net_global_word;
+typedef __attribute__((address_space(3))) uint32_t *net_lds_word;
+
+// A tile of BM = WM MF 16 frames x BN = WN 64 outputs a workgroup; a wavefront MF 16 x 64.  Two stages in LDS of 128 bytes of the
+// reduced axis; while one is multiplied the next is on its way.  x lies in rows of 128 bytes whose 16-byte pieces are exchanged by the
+// row's low bits (piece p of row r holds p ^ (r & 7)), so that 16 rows at once meet no bank twice; W lies as in memory.
+// DMA: x is aligned to 16 bytes and goes to LDS without a register.  A last stage that d_in does not fill goes through registers.
+template <typename T, typename Y, bool DMA, int WM, int WN, int MF>
+__global__ __launch_bounds__(WM * WN * 64)
+void proj_tile_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, int32_t d_in, int32_t chunks, const char *__restrict__ w,
+                      const float *__restrict__ bias, int32_t d_out, const char *__restrict__ b, size_t b_slot, size_t b_part, int32_t rp,
+                      const int32_t *__restrict__ rank, const int32_t *__restrict__ row_slot, const char *__restrict__ h,
+                      Y *__restrict__ y, int64_t y_stride, int32_t tiles_m, int32_t tiles_n)
+{
+    constexpr int E = proj_geo<T>::E, KC = proj_geo<T>::KC, W = WM * WN, BM = WM * MF * 16, XB = BM * 128, WB = WN * 8192, ST = XB + WB;
+    constexpr int XI = BM / 8 / W, WI = WN * 8 / W;         // 1 KB pieces of a stage a wavefront
+    static_assert(XI * W * 8 == BM && WI * W == WN * 8, "a stage is shared evenly");
+    typedef typename proj_geo<T>::frag frag;
+    __shared__ __attribute__((aligned(1024))) char s_buf[2 * ST];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+
+    // neighbouring tiles on one die (workgroups are dealt to the 8 dies in turn), 8 rows of tiles deep: they share x and W in its L2
+    const int n_tiles = tiles_m * tiles_n, per = n_tiles >> 3, more = n_tiles & 7, die = blockIdx.x & 7;
+    const int id = die * per + min(die, more) + (blockIdx.x >> 3);
+    const int strip = id / (8 * tiles_n), deep = min(8, tiles_m - strip * 8), in = id - strip * 8 * tiles_n;
+    const int64_t m0 = (int64_t)(strip * 8 + in % deep) * BM;
+    const int g0 = (in / deep) * WN;                        // first group of 64 outputs
+
+    // where this lane's pieces come from: x at a 32-bit offset from the tile's first row (DMA; the host sees to that), W one offset for all
+    const int xk = ((lane & 7) ^ (lane >> 3)) * E;          // element of the stage (rows of a piece start at a multiple of 8)
+    const char *xt = (const char *)(x + m0 * x_stride);
+    const char *wt = w + (size_t)g0 * chunks * 4096;
+    typedef typename std::conditional<DMA, uint32_t, uint64_t>::type offs;
+    offs xo[XI];
+#pragma unroll
+    for (int i = 0; i < XI; ++i) {
+        const int64_t r = min((int64_t)(wave * XI + i) * 8 + (lane >> 3), (int64_t)rows - 1 - m0);
+        xo[i] = (offs)((r * x_stride + xk) * (int64_t)sizeof(T));
+    }
+    const int stages = chunks / 2;
+    const int full = d_in / (2 * KC);                       // stages that d_in fills: stages or stages - 1
+
+    frag xr[DMA ? 1 : XI];
+    auto fetch = [&](int st, int buf) {
+        char *to = s_buf + buf * ST;
+#pragma unroll
+        for (int i = 0; i < WI; ++i) {
+            const int q = wave * WI + i;                    // [group][8 KB]
+            const char *from = wt + ((size_t)(q >> 3) * chunks * 4096 + (size_t)st * 8192 + (q & 7) * 1024);
+            __builtin_amdgcn_global_load_lds((net_global_word)(from + (uint32_t)lane * 16), (net_lds_word)(to + XB + q * 1024), 16, 0, 0);
+        }
+        const char *from = xt + (size_t)st * 128;
+        if (st < full) {
+#pragma unroll
+            for (int i = 0; i < XI; ++i) {
+                if constexpr (DMA) __builtin_amdgcn_global_load_lds((net_global_word)(from + xo[i]), (net_lds_word)(to + (wave * XI + i) * 1024), 16, 0, 0);
+                else xr[i] = __builtin_bit_cast(frag, *(const net_pack<T, E> *)(from + xo[i]));
+            }
+        } else {
+#pragma unroll 1
+            for (int i = 0; i < XI; ++i) {                  // once a tile
+                const int64_t r = min((int64_t)(wave * XI + i) * 8 + (lane >> 3), (int64_t)rows - 1 - m0);
+                *(frag *)(to + (wave * XI + i) * 1024 + lane * 16) = net_load_chunk(x + (m0 + r) * x_stride, st * 2 * KC + xk, d_in);
+            }
+        }
+    };
+    auto put = [&](int st, int buf) {                       // the pieces that came through registers
+        if constexpr (!DMA) {
+            if (st >= full) return;
+#pragma unroll
+            for (int i = 0; i < XI; ++i) *(frag *)(s_buf + buf * ST + (wave * XI + i) * 1024 + lane * 16) = xr[i];
+        }
+    };
+
+    net_f32x4 acc[MF][4] = {};
+    fetch(0, 0);
+    put(0, 0);
+    for (int st = 0; st < stages; ++st) {
+        __syncthreads();
+        const int buf = st & 1;
+        if (st + 1 < stages) fetch(st + 1, buf ^ 1);
+        const char *from = s_buf + buf * ST;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            frag wf[4], xf[MF];
+#pragma unroll
+            for (int f = 0; f < 4; ++f) wf[f] = *(const frag *)(from + XB + wn * 8192 + (c * 4 + f) * 1024 + lane * 16);
+#pragma unroll
+            for (int m = 0; m < MF; ++m) {
+                const int r = (wm * MF + m) * 16 + (lane & 15);
+                xf[m] = *(const frag *)(from + r * 128 + (((c * 4 + (lane >> 4)) ^ (r & 7)) * 16));
+            }
+#pragma unroll
+            for (int m = 0; m < MF; ++m)
+#pragma unroll
+                for (int f = 0; f < 4; ++f) acc[m][f] = net_mfma(wf[f], xf[m], acc[m][f]);
+        }
+        if (st + 1 < stages) put(st + 1, buf ^ 1);
+    }
+
+    int64_t t[MF];
+#pragma unroll
+    for (int m = 0; m < MF; ++m) t[m] = m0 + (wm * MF + m) * 16 + (lane & 15);
+    int slot[MF];
+#pragma unroll
+    for (int m = 0; m < MF; ++m) slot[m] = t[m] >= rows ? kProjNoRow : row_slot ? row_slot[t[m]] : -1;
+    if (row_slot && b) {
+        const size_t group = (size_t)(g0 + wn) * rp * 64 * sizeof(typename proj_b_type<T>::type);
+        const int s0 = __shfl(slot[0], 0);
+        bool same = true;
+#pragma unroll
+        for (int m = 0; m < MF; ++m) same &= slot[m] == s0;
+        if (__all(same)) {
+            if (s0 >= 0) proj_expand<T, 4, MF>(acc, 0, MF, slot, s0, b, b_slot, b_part, group, (rank[s0] + KC - 1) / KC, rp, h, t);
+        } else {
+#pragma unroll
+            for (int m = 0; m < MF; ++m) {
+                uint64_t todo = __ballot(slot[m] >= 0);
+                while (todo) {
+                    const int s = __shfl(slot[m], __builtin_ctzll(todo));
+                    todo &= ~__ballot(slot[m] == s);
+                    proj_expand<T, 4, MF>(acc, m, m + 1, slot, s, b, b_slot, b_part, group, (rank[s] + KC - 1) / KC, rp, h, t);
+                }
+            }
+        }
+    }
+
+    const int o = (g0 + wn) * 64 + (lane >> 4) * 16;        // this lane's 16 outputs
+    float bo[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) bo[i] = bias[o + i];
+    constexpr int SE = 16 / sizeof(Y);
+#pragma unroll
+    for (int m = 0; m < MF; ++m) {
+        if (slot[m] == kProjNoRow) continue;
+        Y *yr = y + t[m] * y_stride + o;
+#pragma unroll
+        for (int i = 0; i < 16; i += SE) {
+            net_pack<Y, SE> v;
+#pragma unroll
+            for (int j = 0; j < SE; ++j) v.v[j] = net_cast<Y>(acc[m][(i + j) >> 2][(i + j) & 3] + bo[i + j]);
+            if (o + i + SE <= d_out) *(net_pack<Y, SE> *)(yr + i) = v;
+            else
+#pragma unroll
+                for (int j = 0; j < SE; ++j)
+                    if (o + i + j < d_out) yr[i + j] = v.v[j];
+        }
+    }
+}
+
+// ---- the product for few rows -----------------------------------------------------------------------------------------------------
+// MF 16 frames x NF 16 outputs a workgroup, whose wavefronts share the reduced axis; no LDS on the way in (nothing is used twice), all of
+// a wavefront's loads on their way at once.  The adapters' terms are taken by the vector units, a lane one frame and four outputs:
+// neighbouring rows seldom share an adapter here.
+template <typename T, typename Y, int NW, int MF, int NF>
+__global__ __launch_bounds__(NW * 64)
+void proj_few_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, int32_t d_in, int32_t chunks, const char *__restrict__ w,
+                     const float *__restrict__ bias, int32_t d_out, const char *__restrict__ b, size_t b_slot, size_t b_part, int32_t rp,
+                     const int32_t *__restrict__ rank, const int32_t *__restrict__ row_slot, const char *__restrict__ h,
+                     Y *__restrict__ y, int64_t y_stride)
+{
+    constexpr int E = proj_geo<T>::E, KC = proj_geo<T>::KC;
+    typedef typename proj_geo<T>::frag frag;
+    typedef typename proj_b_type<T>::type B;
+    __shared__ net_f32x4 s_part[NW][MF * NF][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t m0 = (int64_t)blockIdx.y * MF * 16;
+    const int n0 = blockIdx.x * NF, g = n0 >> 2, f0 = n0 & 3;
+    const T *xp[MF];
+#pragma unroll
+    for (int m = 0; m < MF; ++m) xp[m] = x + min(m0 + m * 16 + (lane & 15), (int64_t)rows - 1) * x_stride;
+    const frag *wp = (const frag *)(w + (size_t)g * chunks * 4096) + f0 * 64 + lane;
+    net_f32x4 acc[MF][NF] = {};
+#pragma unroll 4
+    for (int c = wave; c < chunks; c += NW) {
+        frag xf[MF], wf[NF];
+#pragma unroll
+        for (int f = 0; f < NF; ++f) wf[f] = wp[(size_t)c * 256 + f * 64];
+#pragma unroll
+        for (int m = 0; m < MF; ++m) xf[m] = net_load_chunk(xp[m], c * KC + (lane >> 4) * E, d_in);
+#pragma unroll
+        for (int m = 0; m < MF; ++m)
+#pragma unroll
+            for (int f = 0; f < NF; ++f) acc[m][f] = net_mfma(wf[f], xf[m], acc[m][f]);
+    }
+#pragma unroll
+    for (int m = 0; m < MF; ++m)
+#pragma unroll
+        for (int f = 0; f < NF; ++f) s_part[wave][m * NF + f][lane] = acc[m][f];
+    __syncthreads();
+    for (int q = wave; q < MF * NF; q += NW) {
+        const int m = q / NF, f = q % NF;
+        const int64_t t = m0 + m * 16 + (lane & 15);
+        const int slot = t >= rows ? kProjNoRow : row_slot ? row_slot[t] : -1;
+        const int ol = (lane >> 4) * 16 + (f0 + f) * 4, o = g * 64 + ol;
+        net_f32x4 v = s_part[0][q][lane];
+        for (int i = 1; i < NW; ++i) v += s_part[i][q][lane];
+        if (slot >= 0 && b) {
+            const int chunks_r = (rank[slot] + KC - 1) / KC;
+            const B *bs = (const B *)(b + slot * b_slot) + (size_t)g * rp * 64 + (f0 + f) * 64 * E;
+            const B *hr = (const B *)h + t * proj_geo<T>::parts * rp;
+            for (int p = 0; p < chunks_r * 4; ++p) {        // E ranks at a time
+                const net_pack<B, E> hi = *(const net_pack<B, E> *)(hr + p * E);
+                net_pack<B, E> lo = {};
+                if constexpr (proj_geo<T>::parts == 2) lo = *(const net_pack<B, E> *)(hr + rp + p * E);
+                float hv[E];
+#pragma unroll
+                for (int e = 0; e < E; ++e) hv[e] = net_f32(hi.v[e]) + (proj_geo<T>::parts == 2 ? net_f32(lo.v[e]) : 0.0f);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const B *bp = bs + ((p >> 2) * 256 + (p & 3) * 16 + (lane >> 4) * 4 + i) * E;
+                    const net_pack<B, E> b1 = *(const net_pack<B, E> *)bp;
+                    net_pack<B, E> b2 = {};
+                    if constexpr (proj_b_type<T>::parts == 2) b2 = *(const net_pack<B, E> *)(bp + b_part / sizeof(B));
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const float be = net_f32(b1.v[e]) + (proj_b_type<T>::parts == 2 ? net_f32(b2.v[e]) : 0.0f);
+                        v[i] = __builtin_fmaf(hv[e], be, v[i]);
+                    }
+                }
+            }
+        }
         if (slot == kProjNoRow) continue;
-        float v = acc[i] + bias[o0 + o];
-        if (slot >= 0)
-            for (int j = 0; j < rank[slot]; ++j) v += h[(size_t)row * rp + j] * net_f32(b[((size_t)slot * np + o0 + o) * rp + j]);
-        y[(size_t)row * y_stride + o0 + o] = net_cast<Y>(v);
+        net_pack<Y, 4> out;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out.v[i] = net_cast<Y>(v[i] + bias[o + i]);
+        Y *yr = y + t * y_stride + o;
+        if (o + 4 <= d_out) *(net_pack<Y, 4> *)yr = out;
+        else
+            for (int i = 0; i < 4; ++i)
+                if (o + i < d_out) yr[i] = out.v[i];
     }
 }
 
 static inline int32_t round_up(int32_t v, int32_t m) { return (v + m - 1) / m * m; }
 
+// the object's device current in a scope
+struct proj_on_device {
+    int cur = -1;
+    explicit proj_on_device(int device) { if (hipGetDevice(&cur) != hipSuccess || cur == device || hipSetDevice(device) != hipSuccess) cur = -1; }
+    ~proj_on_device() { if (cur >= 0) (void)hipSetDevice(cur); }
+};
+
 extern "C" void psgpu_proj_free(psgpu_proj_t *p)
 {
     if (!p) return;
-    int cur = -1;
-    (void)hipGetDevice(&cur);
-    if (cur != p->device) (void)hipSetDevice(p->device);
+    proj_on_device on(p->device);
     (void)hipFree(p->w); (void)hipFree(p->bias); (void)hipFree(p->a); (void)hipFree(p->b); (void)hipFree(p->rank); (void)hipFree(p->scale);
-    if (cur >= 0 && cur != p->device) (void)hipSetDevice(cur);
+    (void)hipFree(p->raw);
     delete p;
 }
 
-// rows x cols elements of es bytes -> [rows_p][cols_p], zeros behind
-static void pad_rows(std::vector<char> &dst, const void *src, size_t rows, size_t cols, size_t rows_p, size_t cols_p, size_t es)
+template <typename T>
+static void proj_lay_w(const psgpu_proj_t *p, const char *raw)
 {
-    dst.assign(rows_p * cols_p * es, 0);
-    for (size_t r = 0; r < rows; ++r) memcpy(dst.data() + r * cols_p * es, (const char *)src + r * cols * es, cols * es);
+    const size_t n = (size_t)p->np * (p->kp / proj_geo<T>::KC) * 4;
+    proj_lay_w_kernel<T><<<(uint32_t)((n + 255) / 256), 256>>>((const T *)raw, p->d_out, p->d_in, p->kp / proj_geo<T>::KC, n, (T *)p->w);
+}
+
+template <typename T>
+static void proj_lay_ab(const psgpu_proj_t *p, int32_t slot, int32_t rank, const char *a, const char *b)
+{
+    const size_t na = p->a_slot / 16, nb = p->b_slot / 16 / proj_b_type<T>::parts;
+    proj_lay_a_kernel<T><<<(uint32_t)((na + 255) / 256), 256>>>((const T *)a, rank, p->d_in, p->rp / 16, na, (T *)(p->a + slot * p->a_slot));
+    proj_lay_b_kernel<T><<<(uint32_t)((nb + 255) / 256), 256>>>((const T *)b, p->d_out, rank, p->rp / proj_geo<T>::KC, nb,
+                                                                (typename proj_b_type<T>::type *)(p->b + slot * p->b_slot));
 }
 
 static int proj_fill(psgpu_proj_t *p, const void *weight, const float *bias)
 {
     const size_t es = net_dtype_size(p->dtype), na = (size_t)p->max_adapters;
-    std::vector<char> buf;
-    pad_rows(buf, weight, p->d_out, p->d_in, p->np, p->kp, es);
-    PSGPU_HIP(hipMalloc((void **)&p->w, buf.size()));
-    PSGPU_HIP(hipMemcpy(p->w, buf.data(), buf.size(), hipMemcpyHostToDevice));
-    buf.assign((size_t)p->np * 4, 0);
-    if (bias) memcpy(buf.data(), bias, (size_t)p->d_out * 4);
-    PSGPU_HIP(hipMalloc((void **)&p->bias, buf.size()));
-    PSGPU_HIP(hipMemcpy(p->bias, buf.data(), buf.size(), hipMemcpyHostToDevice));
-    if (!na) return PSGPU_OK;
-    PSGPU_HIP(hipMalloc((void **)&p->a, na * p->rp * p->kp * es));
-    PSGPU_HIP(hipMalloc((void **)&p->b, na * p->np * p->rp * es));
+    const size_t raw_w = (size_t)p->d_out * p->d_in * es, raw_ab = na ? (size_t)p->max_rank * (p->d_in + p->d_out) * es + 32 : 0;
+    PSGPU_HIP(hipDeviceSynchronize());              // (weights in device memory are whole)
+    PSGPU_HIP(hipMalloc((void **)&p->w, (size_t)p->np * p->kp * es));
+    PSGPU_HIP(hipMalloc((void **)&p->bias, (size_t)p->np * 4));
+    PSGPU_HIP(hipMalloc((void **)&p->raw, raw_w > raw_ab ? raw_w : raw_ab));
+    PSGPU_HIP(hipMemcpy(p->raw, weight, raw_w, hipMemcpyDefault));
+    PSGPU_HIP(hipMemset(p->bias, 0, (size_t)p->np * 4));
+    if (bias) PSGPU_HIP(hipMemcpy(p->bias, bias, (size_t)p->d_out * 4, hipMemcpyDefault));
+    if (p->dtype == PSGPU_DT_F32) proj_lay_w<float>(p, p->raw);
+    else if (p->dtype == PSGPU_DT_F16) proj_lay_w<psg_half>(p, p->raw);
+    else proj_lay_w<psg_bf16>(p, p->raw);
+    PSGPU_HIP(hipGetLastError());
+    PSGPU_HIP(hipDeviceSynchronize());
+    if (!na) {
+        PSGPU_HIP(hipFree(p->raw));
+        p->raw = nullptr;
+        return PSGPU_OK;
+    }
+    PSGPU_HIP(hipMalloc((void **)&p->a, na * p->a_slot));
+    PSGPU_HIP(hipMalloc((void **)&p->b, na * p->b_slot));
     PSGPU_HIP(hipMalloc((void **)&p->rank, na * 4));
     PSGPU_HIP(hipMalloc((void **)&p->scale, na * 4));
-    buf.assign(na * 4, 0);
-    PSGPU_HIP(hipMemcpy(p->rank, buf.data(), na * 4, hipMemcpyHostToDevice));
-    PSGPU_HIP(hipMemcpy(p->scale, buf.data(), na * 4, hipMemcpyHostToDevice));
+    PSGPU_HIP(hipMemset(p->rank, 0, na * 4));
+    PSGPU_HIP(hipMemset(p->scale, 0, na * 4));
+    PSGPU_HIP(hipDeviceSynchronize());
     return PSGPU_OK;
 }
 
@@ -142,36 +571,19 @@ extern "C" int psgpu_proj_create(psgpu_proj_t **out, int32_t dtype, int32_t d_in
     PSGPU_REQUIRE(d_in >= 1 && d_in <= (1 << 20) && d_out >= 1 && d_out <= (1 << 20), "psgpu_proj_create: %d inputs, %d outputs (1..2^20)", d_in, d_out);
     PSGPU_REQUIRE(max_adapters >= 0 && max_adapters <= 65536, "psgpu_proj_create: %d adapters (0..65536)", max_adapters);
     PSGPU_REQUIRE(max_adapters == 0 || (max_rank >= 1 && max_rank <= PSGPU_PROJ_MAX_RANK), "psgpu_proj_create: rank %d (1..%d)", max_rank, PSGPU_PROJ_MAX_RANK);
-    int rc = psgpu_check_device();
+    int device = -1, rc = net_check_device(&device);
     if (rc != PSGPU_OK) return rc;
     psgpu_proj_t *p = new (std::nothrow) psgpu_proj_t;
     if (!p) { psgpu_set_error("psgpu_proj_create: out of memory"); return PSGPU_ENOMEM; }
-    p->device = psgpu_get_device();
+    p->device = device;
     p->dtype = dtype; p->d_in = d_in; p->d_out = d_out; p->max_adapters = max_adapters; p->max_rank = max_adapters ? max_rank : 0;
-    p->kp = round_up(d_in, 64); p->np = round_up(d_out, 256); p->rp = round_up(p->max_rank, 16);
-    try { rc = proj_fill(p, weight, bias); }
-    catch (const std::bad_alloc &) { psgpu_set_error("psgpu_proj_create: out of memory"); rc = PSGPU_ENOMEM; }
+    const int32_t es = (int32_t)net_dtype_size(dtype);
+    p->kp = round_up(d_in, 128 / es); p->np = round_up(d_out, 256); p->rp = round_up(p->max_rank, 64 / es);
+    p->a_slot = (size_t)p->rp * p->kp * es;
+    p->b_slot = (size_t)p->rp * p->np * es * (dtype == PSGPU_DT_F16 ? 2 : 1);
+    rc = proj_fill(p, weight, bias);
     if (rc != PSGPU_OK) { psgpu_proj_free(p); return rc; }
     *out = p;
-    return PSGPU_OK;
-}
-
-static int proj_store_adapter(psgpu_proj_t *p, int32_t slot, int32_t rank, const void *a, const void *b, float scale)
-{
-    const size_t es = net_dtype_size(p->dtype);
-    std::vector<char> ba, bb;
-    if (rank) {
-        pad_rows(ba, a, rank, p->d_in, p->rp, p->kp, es);
-        pad_rows(bb, b, p->d_out, rank, p->np, p->rp, es);
-    }
-    PSGPU_HIP(hipDeviceSynchronize());              // calls that read the slot have ended; later ones see it whole
-    const int32_t none = 0;
-    PSGPU_HIP(hipMemcpy(p->rank + slot, &none, 4, hipMemcpyHostToDevice));      // (a copy that fails leaves the slot empty)
-    if (!rank) return PSGPU_OK;
-    PSGPU_HIP(hipMemcpy(p->a + slot * ba.size(), ba.data(), ba.size(), hipMemcpyHostToDevice));
-    PSGPU_HIP(hipMemcpy(p->b + slot * bb.size(), bb.data(), bb.size(), hipMemcpyHostToDevice));
-    PSGPU_HIP(hipMemcpy(p->scale + slot, &scale, 4, hipMemcpyHostToDevice));
-    PSGPU_HIP(hipMemcpy(p->rank + slot, &rank, 4, hipMemcpyHostToDevice));
     return PSGPU_OK;
 }
 
@@ -184,8 +596,21 @@ extern "C" int psgpu_proj_set_adapter(psgpu_proj_t *p, int32_t slot, int32_t ran
     PSGPU_REQUIRE(rank == 0 || (a && b), "psgpu_proj_set_adapter: NULL argument");
     PSGPU_REQUIRE(rank == 0 || std::isfinite(scale), "psgpu_proj_set_adapter: scale %g", (double)scale);
     PSGPU_REQUIRE(psgpu_get_device() == p->device, "psgpu_proj_set_adapter: the projection lives on device %d, the current one is %d", p->device, psgpu_get_device());
-    try { return proj_store_adapter(p, slot, rank, a, b, scale); }
-    catch (const std::bad_alloc &) { psgpu_set_error("psgpu_proj_set_adapter: out of memory"); return PSGPU_ENOMEM; }
+    const size_t es = net_dtype_size(p->dtype), raw_a = (size_t)rank * p->d_in * es, at_b = (raw_a + 15) / 16 * 16;
+    PSGPU_HIP(hipDeviceSynchronize());              // calls that read the slot have ended; later ones see it whole
+    const int32_t none = 0;
+    PSGPU_HIP(hipMemcpy(p->rank + slot, &none, 4, hipMemcpyHostToDevice));      // (a copy that fails leaves the slot empty)
+    if (!rank) return PSGPU_OK;
+    PSGPU_HIP(hipMemcpy(p->raw, a, raw_a, hipMemcpyDefault));
+    PSGPU_HIP(hipMemcpy(p->raw + at_b, b, (size_t)rank * p->d_out * es, hipMemcpyDefault));
+    if (p->dtype == PSGPU_DT_F32) proj_lay_ab<float>(p, slot, rank, p->raw, p->raw + at_b);
+    else if (p->dtype == PSGPU_DT_F16) proj_lay_ab<psg_half>(p, slot, rank, p->raw, p->raw + at_b);
+    else proj_lay_ab<psg_bf16>(p, slot, rank, p->raw, p->raw + at_b);
+    PSGPU_HIP(hipGetLastError());
+    PSGPU_HIP(hipMemcpy(p->scale + slot, &scale, 4, hipMemcpyHostToDevice));
+    PSGPU_HIP(hipMemcpy(p->rank + slot, &rank, 4, hipMemcpyHostToDevice));
+    PSGPU_HIP(hipDeviceSynchronize());
+    return PSGPU_OK;
 }
 
 extern "C" int32_t psgpu_proj_d_in(const psgpu_proj_t *p) { return p ? p->d_in : PSGPU_EINVAL; }
@@ -200,21 +625,62 @@ extern "C" size_t psgpu_proj_work_bytes(const psgpu_proj_t *p, int32_t total_fra
     return proj_slot_bytes(total_frames) + (size_t)total_frames * p->rp * 4;
 }
 
+template <typename T>
+static void proj_shrink(const psgpu_proj_t *p, const void *x, int64_t xs, const int32_t *off, const int32_t *adapter, int32_t n_utt,
+                        int32_t total, int32_t *slots, char *h, hipStream_t st)
+{
+    const int32_t chunks = p->kp / proj_geo<T>::KC;
+    const char *a = adapter ? p->a : nullptr;
+    // few rows: one a workgroup up to 2048 of them, so that all run at once
+    const bool few = total <= 16384;
+    const int32_t tile = total <= 2048 ? 1 : total <= 8192 ? 4 : 16;
+    const uint32_t grid = few ? (uint32_t)((total + tile - 1) / tile) : (uint32_t)(((int64_t)total + 127) / 128);
+#define SHRINK(RF) do { \
+        if (few) proj_shrink_few_kernel<T, RF><<<grid, 256, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, a, p->a_slot, p->rp, p->rank, p->scale, p->max_adapters, off, adapter, n_utt, tile, slots, h); \
+        else proj_shrink_kernel<T, RF><<<grid, 256, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, a, p->a_slot, p->rp, p->rank, p->scale, p->max_adapters, off, adapter, n_utt, slots, h); \
+    } while (0)
+    if (p->rp <= 16) SHRINK(1);
+    else if (p->rp <= 32) SHRINK(2);
+    else if (p->rp <= 64) SHRINK(4);
+    else SHRINK(8);
+#undef SHRINK
+}
+
 template <typename T, typename Y>
 static void proj_launch(const psgpu_proj_t *p, const void *x, int64_t xs, const int32_t *off, const int32_t *adapter, int32_t n_utt,
                         int32_t total, void *y, int64_t ys, char *work, hipStream_t st)
 {
+    const int32_t chunks = p->kp / proj_geo<T>::KC;
     int32_t *slots = nullptr;
-    float *h = nullptr;
+    char *h = nullptr;
     if (off) {
         slots = (int32_t *)work;
-        h = (float *)(work + proj_slot_bytes(total));
-        proj_shrink_kernel<T><<<(uint32_t)total, 64, 0, st>>>((const T *)x, xs, p->d_in, p->kp, (const T *)p->a, p->rp, p->rank, p->scale,
-                                                              p->max_adapters, off, adapter, n_utt, slots, h);
+        h = work + proj_slot_bytes(total);
+        proj_shrink<T>(p, x, xs, off, adapter, n_utt, total, slots, h, st);
     }
-    const dim3 grid((uint32_t)((p->d_out + kTile - 1) / kTile), (uint32_t)((total + kTile - 1) / kTile));
-    proj_tile_kernel<T, Y><<<grid, 256, 0, st>>>((const T *)x, xs, total, p->d_in, p->kp, (const T *)p->w, p->bias, p->d_out, (const T *)p->b,
-                                                 p->np, p->rp, p->rank, slots, h, (Y *)y, ys);
+    const char *b = adapter ? p->b : nullptr;
+    const size_t b_part = p->b_slot / proj_b_type<T>::parts;
+    const bool dma = (((uintptr_t)x | (uintptr_t)(xs * sizeof(T))) & 15) == 0 && xs < ((int64_t)1 << 30) / 256 / (int64_t)sizeof(T);
+    const int64_t t128 = (((int64_t)total + 127) / 128) * ((p->d_out + 127) / 128), t256 = (((int64_t)total + 255) / 256) * ((p->d_out + 255) / 256);
+#define TILE(D, WM, WN, MF) do { \
+        const int32_t tm = (int32_t)(((int64_t)total + WM * MF * 16 - 1) / (WM * MF * 16)), tn = (p->d_out + WN * 64 - 1) / (WN * 64); \
+        proj_tile_kernel<T, Y, D, WM, WN, MF><<<(uint32_t)tm * (uint32_t)tn, WM * WN * 64, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, p->w, p->bias, p->d_out, \
+            b, p->b_slot, b_part, p->rp, p->rank, slots, h, (Y *)y, ys, tm, tn); \
+    } while (0)
+    if (t128 < 256) {
+        if (total <= 16) {
+            const dim3 grid((uint32_t)((p->d_out + 63) / 64 * 4), 1);
+            proj_few_kernel<T, Y, 4, 1, 1><<<grid, 256, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, p->w, p->bias, p->d_out, b, p->b_slot, b_part, p->rp, p->rank, slots, h, (Y *)y, ys);
+        } else {
+            const dim3 grid((uint32_t)((p->d_out + 63) / 64), (uint32_t)((total + 31) / 32));
+            proj_few_kernel<T, Y, 4, 2, 4><<<grid, 256, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, p->w, p->bias, p->d_out, b, p->b_slot, b_part, p->rp, p->rank, slots, h, (Y *)y, ys);
+        }
+    } else if (sizeof(T) == 4 || t256 < 512) {
+        if (dma) TILE(true, 2, 2, 4); else TILE(false, 2, 2, 4);
+    } else {
+        if constexpr (sizeof(T) == 2) { if (dma) TILE(true, 2, 4, 8); else TILE(false, 2, 4, 8); }
+    }
+#undef TILE
 }
 
 extern "C" int psgpu_proj_run_dev(psgpu_proj_t *p, const void *x_dev, int64_t x_stride, const int32_t *utt_off_dev,
@@ -223,7 +689,7 @@ extern "C" int psgpu_proj_run_dev(psgpu_proj_t *p, const void *x_dev, int64_t x_
 {
     psgpu_clear_error();
     PSGPU_REQUIRE(p, "psgpu_proj_run_dev: NULL argument");
-    PSGPU_REQUIRE(total_frames >= 0 && total_frames <= 65535 * kTile, "psgpu_proj_run_dev: %d frames", total_frames);
+    PSGPU_REQUIRE(total_frames >= 0 && (int64_t)total_frames * ((p->d_out + 127) / 128) <= (int64_t)1 << 37, "psgpu_proj_run_dev: %d frames of %d outputs", total_frames, p->d_out);
     PSGPU_REQUIRE(x_stride >= p->d_in && y_stride >= p->d_out, "psgpu_proj_run_dev: a row stride is below the row's %d inputs or %d outputs", p->d_in, p->d_out);
     PSGPU_REQUIRE(y_dtype == p->dtype || y_dtype == PSGPU_DT_F32, "psgpu_proj_run_dev: y_dtype %d (the projection's own, %d, or 32 bits)", y_dtype, p->dtype);
     PSGPU_REQUIRE(utt_off_dev || !adapter_dev, "psgpu_proj_run_dev: adapters without utterance offsets");
@@ -236,9 +702,10 @@ extern "C" int psgpu_proj_run_dev(psgpu_proj_t *p, const void *x_dev, int64_t x_
     PSGPU_REQUIRE(work_bytes >= need && (work_dev || !need), "psgpu_proj_run_dev: %zu bytes of workspace, psgpu_proj_work_bytes asks for %zu", work_bytes, need);
     PSGPU_REQUIRE(((uintptr_t)work_dev & 15) == 0, "psgpu_proj_run_dev: the workspace is not aligned to 16 bytes");
     PSGPU_REQUIRE(!need || (net_disjoint(x_dev, nx, work_dev, need) && net_disjoint(y_dev, ny, work_dev, need)), "psgpu_proj_run_dev: the workspace overlaps the input or the output");
-    const int rc = psgpu_check_device();
+    int device = -1;
+    const int rc = net_check_device(&device);
     if (rc != PSGPU_OK) return rc;
-    PSGPU_REQUIRE(psgpu_get_device() == p->device, "psgpu_proj_run_dev: the projection lives on device %d, the current one is %d", p->device, psgpu_get_device());
+    PSGPU_REQUIRE(device == p->device, "psgpu_proj_run_dev: the projection lives on device %d, the current one is %d", p->device, device);
     const hipStream_t st = (hipStream_t)stream;
     char *work = (char *)work_dev;
 #define RUN(T, Y) proj_launch<T, Y>(p, x_dev, x_stride, utt_off_dev, adapter_dev, n_utt, total_frames, y_dev, y_stride, work, st)

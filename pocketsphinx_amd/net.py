@@ -64,30 +64,30 @@ def _p(t):
     return C.c_void_p(None if t is None else t.data_ptr())
 
 
-def _host(w, shape_name, dtype=None):
-    """a weight as a contiguous host tensor"""
+def _matrix(w, shape_name, dtype=None):
+    """a weight as a contiguous tensor, where it lies"""
     import torch
     t = w if torch.is_tensor(w) else torch.from_numpy(np.ascontiguousarray(w))
     if t.dim() != 2 or t.dtype not in _dtypes() or (dtype is not None and t.dtype != dtype):
         raise ValueError("%s: a matrix of %s is needed" % (shape_name, dtype if dtype is not None else "float32, float16 or bfloat16"))
-    return t.detach().cpu().contiguous()
+    return t.detach().contiguous()
 
 
 class AdaptedProjection:
     """y[t] = bias + W x[t] + scale_a B_a (A_a x[t]): one projection for all, a low-rank adapter for each utterance (psgpu_proj_*).
 
-    weight [d_out][d_in] (torch or numpy; its type is the layer's), bias [d_out] or None; up to max_adapters adapters of ranks up to
+    weight [d_out][d_in] (torch on the host or the device, or numpy; its type is the layer's), bias [d_out] or None; up to max_adapters adapters of ranks up to
     max_rank are loaded with set_adapter.  The object lives on the device that is current here."""
 
     def __init__(self, weight, bias=None, max_adapters=0, max_rank=64):
         import torch
-        w = _host(weight, "weight [d_out][d_in]")
+        w = _matrix(weight, "weight [d_out][d_in]")
         self.dtype = w.dtype
         self.d_out, self.d_in = int(w.shape[0]), int(w.shape[1])
         self.max_adapters, self.max_rank = int(max_adapters), int(max_rank)
         b = None
         if bias is not None:
-            b = (bias if torch.is_tensor(bias) else torch.from_numpy(np.ascontiguousarray(bias))).detach().float().cpu().contiguous()
+            b = (bias if torch.is_tensor(bias) else torch.from_numpy(np.ascontiguousarray(bias))).detach().float().contiguous()
             if tuple(b.shape) != (self.d_out,):
                 raise ValueError("bias: [%d] is needed" % self.d_out)
         h = C.c_void_p()
@@ -97,13 +97,13 @@ class AdaptedProjection:
         self.device = torch.device("cuda", torch.cuda.current_device())
 
     def set_adapter(self, slot, a, b, scale=1.0):
-        """a [rank][d_in], b [d_out][rank] of the layer's type into a slot; a = b = None empties it.  Waits for the device."""
+        """a [rank][d_in], b [d_out][rank] of the layer's type, on the host or the device, into a slot; a = b = None empties it.  Waits for the device."""
         import torch
         if (a is None) != (b is None):
             raise ValueError("an adapter is a and b")
         rank = 0
         if a is not None:
-            a, b = _host(a, "a [rank][d_in]", self.dtype), _host(b, "b [d_out][rank]", self.dtype)
+            a, b = _matrix(a, "a [rank][d_in]", self.dtype), _matrix(b, "b [d_out][rank]", self.dtype)
             rank = int(a.shape[0])
             if rank < 1 or tuple(a.shape) != (rank, self.d_in) or tuple(b.shape) != (self.d_out, rank):
                 raise ValueError("a [rank][%d] and b [%d][rank] are needed" % (self.d_in, self.d_out))

@@ -182,6 +182,78 @@ def test_projection_large_hidden_values(dtype):
     _close(layer(x.cuda(), _dev([0, 20]), _dev([0])), want, err, DT[dtype], "y")
 
 
+LARGE = [
+    # d_in, d_out, rows (about), elements behind a row: tiles of 128 and of 256 frames, x aligned to 16 bytes or not, a last stage that d_in
+    # does not fill (136 = 2 * 64 + 8) or does (128), a d_in below one stage
+    (136, 5126, 1000, 0),
+    (101, 5126, 1000, 3),
+    (128, 2100, 2500, 8),
+    (136, 5126, 6500, 0),
+    (128, 5126, 6500, 1),
+    (24, 8192, 4300, 0),
+]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("ci", range(len(LARGE)))
+def test_projection_in_large_tiles(ci, dtype):
+    """many frames: tiles with one adapter, with several, with frames of one-frame utterances, frames of no utterance"""
+    d_in, d_out, rows, pad = LARGE[ci]
+    g = torch.Generator().manual_seed(400 + ci)
+    layer, w, b, ad = _layer(g, DT[dtype], d_in, d_out, [16, 0, 40, 3], 40)
+    lens = [rows // 3, 1, 1, 0, 1, 17, rows // 5, 2, 2, 0, 0, 1]
+    off = _off(lens + [rows // 4], start=5)
+    n = off[-1] + 9
+    slots = [0, 2, 0, 1, 3, -1, 2, 3, 0, 2, 2, -1, 3]
+    x = _rand(g, n, d_in, dtype=DT[dtype])
+    want, err = net_ref.proj(x, w, b, ad, off, slots)
+    out = torch.full((n, d_out), 5.0, dtype=DT[dtype], device="cuda")
+    layer(_strided(x, pad), _dev(off), _dev(slots), out=out)
+    _close(out[5:off[-1]], want[5:off[-1]], err[5:off[-1]], DT[dtype], "y")
+    assert (out[:5] == 5.0).all() and (out[off[-1]:] == 5.0).all()
+    if dtype != "f32":
+        _close(layer(_strided(x, pad), _dev(off), _dev(slots), out_dtype=torch.float32)[5:off[-1]], want[5:off[-1]], err[5:off[-1]], torch.float32, "y in 32 bits")
+
+
+def test_projection_keeps_other_rows_from_non_finite_ones_in_large_tiles():
+    g = torch.Generator().manual_seed(410)
+    layer, w, b, ad = _layer(g, torch.bfloat16, 136, 5126, [4, 6], 8)
+    off, slots = _off([1, 400, 900]), [0, 1, 0]
+    x = _rand(g, off[-1], 136, dtype=torch.bfloat16)
+    want, err = net_ref.proj(x, w, b, ad, off, slots)
+    x[7, 135] = float("inf"); x[0, 0] = float("nan"); x[1300, 30] = float("-inf")
+    got = layer(x.cuda(), _dev(off), _dev(slots)).double().cpu()
+    mask = torch.ones(off[-1], dtype=torch.bool)
+    mask[[0, 7, 1300]] = False
+    _close(got[mask], want[mask], err[mask], torch.bfloat16, "finite rows")
+    assert torch.isnan(got[0]).all() and not torch.isfinite(got[7]).any() and not torch.isfinite(got[1300]).any()
+
+
+@pytest.mark.parametrize("lens", [[1] * 300, [0] * 200 + [1] * 3 + [0] * 500 + [2] * 70, [1] * 5000, [0, 0, 1]])
+def test_projection_finds_the_utterance_of_every_row(lens):
+    """many utterances, runs of empty ones: each row its own adapter's factor"""
+    layer = AdaptedProjection(torch.zeros(16, 8), None, max_adapters=97, max_rank=1)
+    for s in range(97):
+        layer.set_adapter(s, torch.ones(1, 8), torch.ones(16, 1), float(s + 1))
+    off = _off(lens)
+    slots = [(31 * u) % 97 for u in range(len(lens))]
+    y = layer(torch.ones(off[-1], 8, device="cuda"), _dev(off), _dev(slots)).cpu()
+    want = torch.tensor([8.0 * (slots[u] + 1) for u, n in enumerate(lens) for _ in range(n)])
+    assert torch.equal(y, want[:, None].expand(-1, 16))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_projection_takes_weights_from_the_device(dtype):
+    g = torch.Generator().manual_seed(420)
+    w, b = _rand(g, 70, 40, dtype=DT[dtype]), _rand(g, 70)
+    a, bb = _rand(g, 5, 40, dtype=DT[dtype]), _rand(g, 70, 5, dtype=DT[dtype])
+    one, two = AdaptedProjection(w, b, 1, 8), AdaptedProjection(w.cuda(), b.cuda(), 1, 8)
+    one.set_adapter(0, a, bb, 0.5)
+    two.set_adapter(0, a.cuda(), bb.t().contiguous().cuda().t(), 0.5)
+    x = _rand(g, 33, 40, dtype=DT[dtype]).cuda()
+    assert torch.equal(one(x, _dev([0, 33]), _dev([0])), two(x, _dev([0, 33]), _dev([0])))
+
+
 def test_projection_refusals():
     w = torch.zeros(8, 16, dtype=torch.bfloat16)
     layer = AdaptedProjection(w, None, max_adapters=2, max_rank=4)
