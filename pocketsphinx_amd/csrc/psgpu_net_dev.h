@@ -56,6 +56,10 @@ __device__ __forceinline__ int net_utt_of_rows(const int32_t *off, int n_utt, in
     return u >= 0 && u < n_utt && off[u] <= row && off[u + 1] > row ? u : -1;
 }
 
+// Waits for this wavefront's loads (vmcnt 0, the other counters left alone).  Loads that go to LDS without a register need it in front of
+// the barrier that hands them to other wavefronts: the barrier's own wait covers LDS instructions, not always these.
+__device__ __forceinline__ void net_wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+
 // ---- matrix instructions ------------------------------------------------------------------------------------------------------------
 // Products of 16 x 16 from 16 bytes a lane: lane l of the first operand holds row l & 15, of the second column l & 15, elements
 // (l >> 4) * E .. + E - 1 of the reduced axis (E = 16 bytes of T; one instruction of 4 E elements for halves, four of 4 for floats, which

@@ -340,6 +340,7 @@ void proj_tile_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, i
     fetch(0, 0);
     put(0, 0);
     for (int st = 0; st < stages; ++st) {
+        net_wait_loads();                                   // this wavefront's pieces of the stage lie in LDS; the barrier: everybody's
         __syncthreads();
         const int buf = st & 1;
         if (st + 1 < stages) fetch(st + 1, buf ^ 1);

@@ -215,6 +215,33 @@ def test_projection_in_large_tiles(ci, dtype):
         _close(layer(_strided(x, pad), _dev(off), _dev(slots), out_dtype=torch.float32)[5:off[-1]], want[5:off[-1]], err[5:off[-1]], torch.float32, "y in 32 bits")
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("pad", [0, 3])
+@pytest.mark.parametrize("rows, d_in, d_out", [(20000, 1000, 2100), (4300, 1024, 8192), (2500, 2048, 1024)])
+def test_projection_over_many_stages(rows, d_in, d_out, pad, dtype):
+    """a long reduced axis in large tiles: every stage is whole before it is multiplied (64-bit products on the device)"""
+    g = torch.Generator().manual_seed(430)
+    layer, w, b, ad = _layer(g, DT[dtype], d_in, d_out, [24, 7], 24)
+    off, slots = [0, rows // 2 + 3, rows], [0, 1]
+    x = _rand(g, rows, d_in, dtype=DT[dtype])
+    xd, wd = x.cuda().double(), w.cuda().double()
+    want = xd @ wd.t() + b.cuda().double()
+    mag = xd.abs() @ wd.abs().t() + b.cuda().double().abs()
+    err = torch.zeros_like(want)
+    for u, s in enumerate(slots):               # as net_ref.proj
+        a, bb, sc = (v.cuda().double() if torch.is_tensor(v) else v for v in ad[s])
+        r = slice(off[u], off[u + 1])
+        h = sc * (xd[r] @ a.t())
+        want[r] += h @ bb.t()
+        mag[r] += h.abs() @ bb.abs().t()
+        err[r] = (sc * (xd[r].abs() @ a.abs().t()) * (2 * net_ref.U * (d_in + 1)) + h.abs() * (2.0 ** -16 + 2.0 ** -17)) @ bb.abs().t()
+        err[r] += 2 * net_ref.U * (d_in + 1 + 3 * a.shape[0]) * mag[r]
+    want, err = want.cpu(), err.cpu()
+    xs = _strided(x, pad)
+    for _ in range(3):
+        _close(layer(xs, _dev(off), _dev(slots)), want, err, DT[dtype], "y")
+
+
 def test_projection_keeps_other_rows_from_non_finite_ones_in_large_tiles():
     g = torch.Generator().manual_seed(410)
     layer, w, b, ad = _layer(g, torch.bfloat16, 136, 5126, [4, 6], 8)
