@@ -5,58 +5,421 @@
 //
 // What cmn() with -varnorm is for cepstra (reference src/feat/cmn.c:166-233), per group of channels and with a learned scale.
 // Sums run in 64 bits: sum x^2 - n m^2 then keeps its digits for groups whose mean is far above their spread.
+//
+// Every kernel works on a slice of whole neighbouring groups of some rows: a work-item has one chunk of 16 bytes of the slice's
+// channels and every nrl-th row, so a wavefront reads rows in one piece at any alignment.  Memory bounds them all.
 #include "psgpu_net_dev.h"
 #include <cmath>
 
-constexpr int kGnThreads = 256;
+struct gn_args {
+    const void *x;
+    int64_t xs;
+    const int32_t *off;
+    int32_t n_utt, total, n_chan, per, n_groups, gs;    // gs: groups a slice
+    const float *weight, *bias;
+    float eps;
+    void *y;
+    int64_t ys;
+    double2 *part;                                      // [tiles + n_utt][n_groups] sums of a tile's rows of an utterance
+    int32_t tile_rows;
+};
 
-__device__ __forceinline__ float gn_act(int act, float v)
+struct gn_stat { float mhi, mlo, rstd; };               // the mean in two parts
+
+// 1 - (the normal distribution's integral up to t >= 0) = exp(-t^2 / 2) s P(s), s = 1 / (1 + 0.21 t): P a least-maximum fit of its
+// relative error over 0 <= t <= 14 (1.6e-8), beyond which the result is 0 in 32 bits.  erff() took three times the instructions and
+// bound the kernel.
+__device__ __forceinline__ float gn_upper_tail(float t)
 {
-    switch (act) {
+    const float s = __builtin_amdgcn_rcpf(__builtin_fmaf(0.21f, t, 1.0f));
+    float p = -0.07165627723f;
+    p = __builtin_fmaf(p, s, 0.2835884168f);
+    p = __builtin_fmaf(p, s, -0.3302530846f);
+    p = __builtin_fmaf(p, s, 0.3494006789f);
+    p = __builtin_fmaf(p, s, -0.09392498913f);
+    p = __builtin_fmaf(p, s, 0.1248726401f);
+    p = __builtin_fmaf(p, s, 0.0691921909f);
+    p = __builtin_fmaf(p, s, 0.08506885524f);
+    p = __builtin_fmaf(p, s, 0.08371157581f);
+    return __builtin_amdgcn_exp2f(t * t * -0.72134752044448170f) * (s * p);
+}
+
+template <int ACT>
+__device__ __forceinline__ float gn_act(float v)
+{
+    switch (ACT) {
     case PSGPU_ACT_RELU: return v < 0.0f ? 0.0f : v;                              // (a NaN stays one)
-    case PSGPU_ACT_SILU: return v / (1.0f + expf(-v));
-    case PSGPU_ACT_GELU: return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
+    case PSGPU_ACT_SILU: return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f));
+    case PSGPU_ACT_GELU: {
+        const float q = gn_upper_tail(fabsf(v));
+        return v * (v < 0.0f ? q : 1.0f - q);
+    }
     default: return v;
     }
 }
 
-template <typename T>
-__global__ __launch_bounds__(kGnThreads)
-void gnorm_group_kernel(const T *x, int64_t x_stride, const int32_t *__restrict__ utt_off, int32_t total, int32_t n_chan, int32_t per,
-                        const float *__restrict__ weight, const float *__restrict__ bias, float eps, int act, T *y, int64_t y_stride)
+// E channels of a row from c on, zeros from c1 on, as they lie in four registers
+// (FULL: no chunk reaches beyond c1)
+template <bool FULL, typename T>
+__device__ __forceinline__ net_u32x4 gn_load(const T *row, int c, int c1)
 {
-    __shared__ double s_sum[kGnThreads / 64], s_sq[kGnThreads / 64];
-    const int u = blockIdx.y, c0 = blockIdx.x * per, tid = threadIdx.x;
-    const int t0 = max(utt_off[u], 0), t1 = min(utt_off[u + 1], total);
-    if (t1 <= t0) return;
-    const int64_t n = (int64_t)(t1 - t0) * per;
-    double sum = 0.0, sq = 0.0;
-    for (int64_t i = tid; i < n; i += kGnThreads) {
-        const double v = (double)net_f32(x[(t0 + i / per) * x_stride + c0 + i % per]);
-        sum += v;
-        sq += v * v;
-    }
-    for (int o = 32; o; o >>= 1) { sum += __shfl_xor(sum, o); sq += __shfl_xor(sq, o); }
-    if ((tid & 63) == 0) { s_sum[tid >> 6] = sum; s_sq[tid >> 6] = sq; }
-    __syncthreads();
-    sum = sq = 0.0;
-    for (int w = 0; w < kGnThreads / 64; ++w) { sum += s_sum[w]; sq += s_sq[w]; }
-    const double mean = sum / (double)n;
-    double var = sq / (double)n - mean * mean;
-    if (var < 0.0) var = 0.0;                       // (a NaN stays one)
-    const float rstd = (float)(1.0 / sqrt(var + (double)eps)), mhi = (float)mean, mlo = (float)(mean - (double)mhi);
-    for (int64_t i = tid; i < n; i += kGnThreads) {
-        const int64_t t = t0 + i / per;
-        const int c = c0 + (int)(i % per);
-        float v = ((net_f32(x[t * x_stride + c]) - mhi) - mlo) * rstd;
-        v = v * (weight ? weight[c] : 1.0f) + (bias ? bias[c] : 0.0f);
-        y[t * y_stride + c] = net_cast<T>(gn_act(act, v));
+    if constexpr (FULL) return __builtin_bit_cast(net_u32x4, *(const net_pack<T, 16 / sizeof(T)> *)(row + c));
+    else return __builtin_bit_cast(net_u32x4, net_load_chunk(row, c, c1));
+}
+
+// K pairs of sums of a chunk: one for all its channels (they are of one group), or one a channel
+template <typename T, int K>
+__device__ __forceinline__ void gn_add(double (&sum)[K], double (&sq)[K], const net_u32x4 &v)
+{
+#pragma unroll
+    for (int e = 0; e < 16 / (int)sizeof(T); ++e) {
+        const double d = (double)net_elem<T>(v, e);
+        sum[K == 1 ? 0 : e] += d;
+        sq[K == 1 ? 0 : e] = __builtin_fma(d, d, sq[K == 1 ? 0 : e]);
     }
 }
 
+// A slice's place: channels c0 .. c1 - 1 = groups g0 .. g0 + ng - 1; this work-item's row and chunk in it.  A slice of one group may
+// be wider than the workgroup's chunks; its work-items then take it in strides of NT chunks.
+template <typename T, int NT>
+struct gn_place {
+    int g0, ng, c0, c1, cw, nrl, rl, ck;
+    __device__ __forceinline__ gn_place(const gn_args &a, int slice)
+    {
+        constexpr int E = 16 / sizeof(T);
+        g0 = slice * a.gs;
+        ng = min(a.gs, a.n_groups - g0);
+        c0 = g0 * a.per;
+        c1 = c0 + ng * a.per;
+        cw = min((c1 - c0 + E - 1) / E, NT);
+        nrl = NT / cw;
+        rl = (int)threadIdx.x / cw;
+        ck = (int)threadIdx.x - rl * cw;
+        if (rl >= nrl) rl = 0x7fffffff;                  // no row is its own
+    }
+};
+
+// sums over the lanes of `lanes` (a power of two) neighbours, to all of them
+__device__ __forceinline__ void gn_sum_lanes(double &sum, double &sq, int lanes)
+{
+    for (int o = lanes >> 1; o; o >>= 1) { sum += __shfl_xor(sum, o); sq += __shfl_xor(sq, o); }
+}
+
+// the slice's groups: group tid / lanes (may be beyond ng) is summed by `lanes` neighbours
+template <int NT>
+__device__ __forceinline__ int gn_lanes(int ng)
+{
+    int l = 64;
+    while (l > 1 && l * ng > NT) l >>= 1;
+    return l;
+}
+
+// the work-items' sums joined by groups, in one order always.  s_red [NT * K]; every work-item calls it; lane 0 of a group's lanes has
+// the result where its group is one (returns it, else -1)
+template <typename T, int NT, int K>
+__device__ __forceinline__ int gn_join(const gn_args &a, const gn_place<T, NT> &p, double (&sum)[K], double (&sq)[K], double2 *s_red, double2 &out)
+{
+    constexpr int E = 16 / sizeof(T);
+    const int tid = threadIdx.x;
+#pragma unroll
+    for (int k = 0; k < K; ++k) s_red[tid * K + k] = make_double2(sum[k], sq[k]);
+    __syncthreads();
+    const int lanes = gn_lanes<NT>(p.ng), g = tid / lanes, lane = tid & (lanes - 1);
+    double s = 0.0, q = 0.0;
+    if (g < p.ng) {
+        const int n = K > 1 ? a.per : p.ng == 1 ? p.cw : a.per / E;             // a group's pairs in a row of work-items
+        const int at = K > 1 ? g * a.per : g * n;
+        if (p.nrl >= n) {
+            for (int r = lane; r < p.nrl; r += lanes)
+                for (int i = 0; i < n; ++i) {
+                    const double2 v = s_red[r * p.cw * K + at + i];
+                    s += v.x; q += v.y;
+                }
+        } else {
+            for (int r = 0; r < p.nrl; ++r)
+                for (int i = lane; i < n; i += lanes) {
+                    const double2 v = s_red[r * p.cw * K + at + i];
+                    s += v.x; q += v.y;
+                }
+        }
+    }
+    gn_sum_lanes(s, q, lanes);
+    out = make_double2(s, q);
+    return g < p.ng && lane == 0 ? g : -1;
+}
+
+__device__ __forceinline__ gn_stat gn_finish(double2 s, double n, float eps)
+{
+    const double mean = s.x / n;
+    double var = s.y / n - mean * mean;
+    if (var < 0.0) var = 0.0;                           // (a NaN stays one)
+    gn_stat r;
+    r.rstd = (float)(1.0 / sqrt(var + (double)eps));
+    r.mhi = (float)mean;
+    r.mlo = (float)(mean - (double)r.mhi);
+    return r;
+}
+
+// what a chunk's channels are multiplied by and what is added
+template <int E> struct gn_affine { float mhi[E], mlo[E], rw[E], b[E]; };
+
+template <typename T, int NT, int K>
+__device__ __forceinline__ void gn_affine_of(const gn_args &a, const gn_place<T, NT> &p, int c, const gn_stat *s_stat, gn_affine<16 / sizeof(T)> &f)
+{
+    constexpr int E = 16 / sizeof(T);
+    const int g1 = min((c - p.c0) / a.per, p.ng - 1);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int ce = min(c + e, p.c1 - 1);
+        const gn_stat s = s_stat[K == 1 || p.ng == 1 ? g1 : (ce - p.c0) / a.per];
+        f.mhi[e] = s.mhi;
+        f.mlo[e] = s.mlo;
+        f.rw[e] = a.weight ? s.rstd * a.weight[ce] : s.rstd;
+        f.b[e] = a.bias ? a.bias[ce] : 0.0f;
+    }
+}
+
+template <typename T, int ACT, bool FULL>
+__device__ __forceinline__ void gn_store(const net_u32x4 &v, const gn_affine<16 / sizeof(T)> &f, T *row, int c, int c1)
+{
+    constexpr int E = 16 / sizeof(T);
+    net_pack<T, E> o;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o.v[e] = net_cast<T>(gn_act<ACT>(__builtin_fmaf((net_elem<T>(v, e) - f.mhi[e]) - f.mlo[e], f.rw[e], f.b[e])));
+    if (FULL || c + E <= c1) *(net_pack<T, E> *)(row + c) = o;
+    else
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (c + e < c1) row[c + e] = o.v[e];
+}
+
+// ---- an utterance's slice a workgroup ----------------------------------------------------------------------------------------------
+// The first NCH chunks of a work-item stay in registers from the sums to the result: what fits there is read once.
+template <typename T, int NT, int NCH, int K, bool FULL, int ACT>
+__global__ __launch_bounds__(NT, 4)
+void gnorm_held_kernel(gn_args a)
+{
+    constexpr int E = 16 / sizeof(T);
+    __shared__ double2 s_red[NT * K];
+    __shared__ gn_stat s_stat[NT];
+    const int u = blockIdx.y;
+    const int t0 = max(a.off[u], 0), t1 = min(a.off[u + 1], a.total);
+    if (t1 <= t0) return;
+    const gn_place<T, NT> p(a, blockIdx.x);
+    const T *x = (const T *)a.x;
+    T *y = (T *)a.y;
+    const int len = t1 - t0, c = p.c0 + p.ck * E;
+    // rows rl + i nrl, i < mine; at 32-bit offsets from the utterance's first (the host sees to that)
+    const int mine = p.rl < len ? (len - 1 - p.rl) / p.nrl + 1 : 0;
+    const char *xu = (const char *)(x + t0 * a.xs);
+    const uint32_t x0 = mine ? (uint32_t)(p.rl * (int)a.xs) * sizeof(T) : 0, x_step = (uint32_t)(p.nrl * (int)a.xs) * sizeof(T);
+    net_u32x4 held[NCH];
+    double sum[K] = {}, sq[K] = {};
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        held[i] = {};
+        if (i < mine) held[i] = gn_load<FULL>((const T *)(xu + (x0 + i * x_step)), c, p.c1);
+    }
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        gn_add<T, K>(sum, sq, held[i]);
+        __builtin_amdgcn_sched_barrier(0);              // (or all chunks are widened to 64 bits before the first sum)
+    }
+    const bool wide = c + NT * E < p.c1 && p.nrl == 1;          // one group, wider than the workgroup
+    const int64_t behind = (int64_t)p.rl + (int64_t)NCH * p.nrl;
+    for (int64_t r = behind; r < len; r += p.nrl) gn_add<T, K>(sum, sq, gn_load<FULL>(x + (t0 + r) * a.xs, c, p.c1));
+    if (wide)
+        for (int64_t r = p.rl; r < len; ++r)
+            for (int cc = c + NT * E; cc < p.c1; cc += NT * E) gn_add<T, K>(sum, sq, gn_load<FULL>(x + (t0 + r) * a.xs, cc, p.c1));
+    double2 tot;
+    const int g = gn_join<T, NT, K>(a, p, sum, sq, s_red, tot);
+    if (g >= 0) s_stat[g] = gn_finish(tot, (double)len * a.per, a.eps);
+    __syncthreads();
+    if (p.rl >= len || c >= p.c1) return;
+    gn_affine<E> f;
+    gn_affine_of<T, NT, K>(a, p, c, s_stat, f);
+    // kept as they lie in memory: without this the compiler keeps every element unpacked from the sums on
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) asm volatile("" : "+v"(held[i]));
+    char *yu = (char *)(y + t0 * a.ys);
+    const uint32_t y0 = (uint32_t)(p.rl * (int)a.ys) * sizeof(T), y_step = (uint32_t)(p.nrl * (int)a.ys) * sizeof(T);
+#pragma unroll
+    for (int i = 0; i < NCH; ++i)
+        if (i < mine) gn_store<T, ACT, FULL>(held[i], f, (T *)(yu + (y0 + i * y_step)), c, p.c1);
+    for (int64_t r = behind; r < len; r += p.nrl) gn_store<T, ACT, FULL>(gn_load<FULL>(x + (t0 + r) * a.xs, c, p.c1), f, y + (t0 + r) * a.ys, c, p.c1);
+    if (wide)
+        for (int cc = c + NT * E; cc < p.c1; cc += NT * E) {
+            gn_affine_of<T, NT, K>(a, p, cc, s_stat, f);
+            for (int64_t r = p.rl; r < len; ++r) gn_store<T, ACT, FULL>(gn_load<FULL>(x + (t0 + r) * a.xs, cc, p.c1), f, y + (t0 + r) * a.ys, cc, p.c1);
+        }
+}
+
+// ---- tiles of rows, in two passes ----------------------------------------------------------------------------------------------------
+// Rows row .. tile_end - 1 begin in which utterance, and how far it reaches; false: no more utterances in the tile.  Partial sums lie
+// at tile + utterance: along the rows one of the two grows from piece to piece, so every piece has a place of its own.
+__device__ __forceinline__ bool gn_next(const gn_args &a, int &row, int tile_end, int &u, int &end)
+{
+    while (row < tile_end) {
+        u = __builtin_amdgcn_readfirstlane(net_utt_of_rows(a.off, a.n_utt, row));
+        if (u >= 0) {
+            end = min(a.off[u + 1], tile_end);
+            return true;
+        }
+        const int first = a.off[0];
+        if (first <= row) return false;
+        row = first;
+    }
+    return false;
+}
+
+template <typename T, int NT, int K, bool FULL>
+__global__ __launch_bounds__(NT)
+void gnorm_sums_kernel(gn_args a)
+{
+    constexpr int E = 16 / sizeof(T);
+    __shared__ double2 s_red[NT * K];
+    const gn_place<T, NT> p(a, blockIdx.x);
+    const int tile = blockIdx.y;
+    const int tile_end = (int)min(((int64_t)tile + 1) * a.tile_rows, (int64_t)a.total);
+    int row = tile * a.tile_rows, u, end;
+    const T *x = (const T *)a.x;
+    while (gn_next(a, row, tile_end, u, end)) {
+        double sum[K] = {}, sq[K] = {};
+        for (int c = p.c0 + p.ck * E; c < p.c1; c += NT * E) {
+            int64_t r = (int64_t)row + p.rl;
+            for (; r + 3 * p.nrl < end; r += 4 * p.nrl) {
+                net_u32x4 v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = gn_load<FULL>(x + (r + i * p.nrl) * a.xs, c, p.c1);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) gn_add<T, K>(sum, sq, v[i]);
+            }
+            for (; r < end; r += p.nrl) gn_add<T, K>(sum, sq, gn_load<FULL>(x + r * a.xs, c, p.c1));
+        }
+        double2 tot;
+        const int g = gn_join<T, NT, K>(a, p, sum, sq, s_red, tot);
+        if (g >= 0) a.part[((size_t)tile + u) * a.n_groups + p.g0 + g] = tot;
+        __syncthreads();
+        row = end;
+    }
+}
+
+template <typename T, int NT, int K, bool FULL, int ACT>
+__global__ __launch_bounds__(NT, 4)
+void gnorm_apply_kernel(gn_args a)
+{
+    constexpr int E = 16 / sizeof(T);
+    __shared__ gn_stat s_stat[NT];
+    const gn_place<T, NT> p(a, blockIdx.x);
+    // the last tiles of the first pass are the first here: the caches may still hold them
+    const int tile = gridDim.y - 1 - blockIdx.y;
+    const int tile_end = (int)min(((int64_t)tile + 1) * a.tile_rows, (int64_t)a.total);
+    int row = tile * a.tile_rows, u, end;
+    const T *x = (const T *)a.x;
+    T *y = (T *)a.y;
+    const int lanes = gn_lanes<NT>(p.ng), g = (int)threadIdx.x / lanes, lane = threadIdx.x & (lanes - 1);
+    while (gn_next(a, row, tile_end, u, end)) {
+        const int t0 = max(a.off[u], 0), t1 = min(a.off[u + 1], a.total);
+        const int i0 = t0 / a.tile_rows, i1 = (t1 - 1) / a.tile_rows;
+        double s = 0.0, q = 0.0;
+        if (g < p.ng)
+            for (int i = i0 + lane; i <= i1; i += lanes) {
+                const double2 v = a.part[((size_t)i + u) * a.n_groups + p.g0 + g];
+                s += v.x; q += v.y;
+            }
+        gn_sum_lanes(s, q, lanes);
+        if (g < p.ng && lane == 0) s_stat[g] = gn_finish(make_double2(s, q), (double)(t1 - t0) * a.per, a.eps);
+        __syncthreads();
+        for (int c = p.c0 + p.ck * E; c < p.c1 && p.rl < end - row; c += NT * E) {
+            gn_affine<E> f;
+            gn_affine_of<T, NT, K>(a, p, c, s_stat, f);
+            int64_t r = (int64_t)row + p.rl;
+            for (; r + 3 * p.nrl < end; r += 4 * p.nrl) {
+                net_u32x4 v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = gn_load<FULL>(x + (r + i * p.nrl) * a.xs, c, p.c1);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) gn_store<T, ACT, FULL>(v[i], f, y + (r + i * p.nrl) * a.ys, c, p.c1);
+            }
+            for (; r < end; r += p.nrl) gn_store<T, ACT, FULL>(gn_load<FULL>(x + r * a.xs, c, p.c1), f, y + r * a.ys, c, p.c1);
+        }
+        __syncthreads();
+        row = end;
+    }
+}
+
+// ---- which way ---------------------------------------------------------------------------------------------------------------------
+constexpr int kGnTiles = 2048;
+
+// rows of a tile: about kGnTiles tiles, of 16 rows or more
+static inline int32_t gn_tile_rows(int32_t total) { const int32_t r = (int32_t)(((int64_t)total + kGnTiles - 1) / kGnTiles); return r < 16 ? 16 : (r + 15) / 16 * 16; }
+
 extern "C" size_t psgpu_group_norm_work_bytes(int32_t n_utt, int32_t total_frames, int32_t n_groups)
 {
-    return 0;
+    if (n_utt <= 0 || total_frames <= 0 || n_groups <= 0) return 0;
+    const int32_t rows = gn_tile_rows(total_frames);
+    return ((size_t)((total_frames - 1) / rows + 1) + (size_t)n_utt) * (size_t)n_groups * sizeof(double2);
+}
+
+// the groups a slice may have so that its chunks are at most nt, and (one statistic a work-item to keep) its groups at most nt
+static int32_t gn_slice(int32_t n_groups, int32_t per, int e, int nt)
+{
+    int64_t gs = (int64_t)nt * e / per;
+    if (gs > nt) gs = nt;
+    if (gs > n_groups) gs = n_groups;
+    return gs < 1 ? 1 : (int32_t)gs;
+}
+
+template <typename T, int ACT>
+static void gn_run(gn_args a, hipStream_t st)
+{
+    constexpr int E = 16 / sizeof(T);
+    const int64_t mean_len = ((int64_t)a.total + a.n_utt - 1) / a.n_utt;
+    const bool one = a.per % E == 0;                    // a chunk lies in one group
+    int64_t gs = gn_slice(a.n_groups, a.per, E, 256);
+    auto chunks = [&](int64_t g) { return mean_len * ((g * a.per + E - 1) / E); };      // of an utterance's slice of g groups
+    auto slices = [&](int64_t g) { return (a.n_groups + g - 1) / g; };
+    // One launch where an utterance's group fits a workgroup's registers on average and there are enough of them: 256 work-items hold
+    // 8 chunks each, 512 hold 24.
+    const bool near_rows = a.xs < 1 << 16 && a.ys < 1 << 16;       // 512 x 24 rows of them lie within 2^32 bytes
+    if (near_rows && chunks(1) <= 256 * 8 && ((int64_t)a.total * a.n_chan <= 1 << 17 || (int64_t)a.n_utt * a.n_groups >= 256)) {
+        while (gs > 1 && (chunks(gs) > 256 * 8 || a.n_utt * slices(gs) < 512)) gs = (gs + 1) / 2;
+        a.gs = (int32_t)gs;
+        const dim3 grid((uint32_t)slices(gs), (uint32_t)a.n_utt);
+        if (one) gnorm_held_kernel<T, 256, 8, 1, true, ACT><<<grid, 256, 0, st>>>(a);
+        else if (gs == 1) gnorm_held_kernel<T, 256, 8, 1, false, ACT><<<grid, 256, 0, st>>>(a);
+        else gnorm_held_kernel<T, 256, 8, E, false, ACT><<<grid, 256, 0, st>>>(a);
+        return;
+    }
+    if (near_rows && one && chunks(1) <= 512 * 24 && (int64_t)a.n_utt * a.n_groups >= 512) {
+        a.gs = 1;
+        gnorm_held_kernel<T, 512, 24, 1, true, ACT><<<dim3((uint32_t)a.n_groups, (uint32_t)a.n_utt), 512, 0, st>>>(a);
+        return;
+    }
+    a.gs = (int32_t)gs;
+    a.tile_rows = gn_tile_rows(a.total);
+    const dim3 grid((uint32_t)slices(gs), (uint32_t)((a.total - 1) / a.tile_rows + 1));
+    if (one) {
+        gnorm_sums_kernel<T, 256, 1, true><<<grid, 256, 0, st>>>(a);
+        gnorm_apply_kernel<T, 256, 1, true, ACT><<<grid, 256, 0, st>>>(a);
+    } else if (gs == 1) {
+        gnorm_sums_kernel<T, 256, 1, false><<<grid, 256, 0, st>>>(a);
+        gnorm_apply_kernel<T, 256, 1, false, ACT><<<grid, 256, 0, st>>>(a);
+    } else {
+        gnorm_sums_kernel<T, 256, E, false><<<grid, 256, 0, st>>>(a);
+        gnorm_apply_kernel<T, 256, E, false, ACT><<<grid, 256, 0, st>>>(a);
+    }
+}
+
+template <typename T>
+static void gn_run_act(const gn_args &a, int32_t act, hipStream_t st)
+{
+    switch (act) {
+    case PSGPU_ACT_RELU: gn_run<T, PSGPU_ACT_RELU>(a, st); break;
+    case PSGPU_ACT_SILU: gn_run<T, PSGPU_ACT_SILU>(a, st); break;
+    case PSGPU_ACT_GELU: gn_run<T, PSGPU_ACT_GELU>(a, st); break;
+    default: gn_run<T, PSGPU_ACT_NONE>(a, st);
+    }
 }
 
 extern "C" int psgpu_group_norm_dev(int32_t dtype, const void *x_dev, int64_t x_stride, const int32_t *utt_off_dev, int32_t n_utt,
@@ -67,30 +430,28 @@ extern "C" int psgpu_group_norm_dev(int32_t dtype, const void *x_dev, int64_t x_
     psgpu_clear_error();
     PSGPU_REQUIRE(net_dtype_ok(dtype), "psgpu_group_norm_dev: dtype %d", dtype);
     PSGPU_REQUIRE(n_utt >= 0 && n_utt <= 65535 && total_frames >= 0, "psgpu_group_norm_dev: %d frames of %d utterances (at most 65535)", total_frames, n_utt);
-    PSGPU_REQUIRE(n_chan >= 1 && n_groups >= 1 && n_chan % n_groups == 0, "psgpu_group_norm_dev: %d channels in %d groups", n_chan, n_groups);
+    PSGPU_REQUIRE(n_chan >= 1 && n_chan <= (1 << 30) && n_groups >= 1 && n_chan % n_groups == 0, "psgpu_group_norm_dev: %d channels in %d groups", n_chan, n_groups);
     PSGPU_REQUIRE(x_stride >= n_chan && y_stride >= n_chan, "psgpu_group_norm_dev: a row stride is below %d", n_chan);
     PSGPU_REQUIRE(act >= PSGPU_ACT_NONE && act <= PSGPU_ACT_GELU, "psgpu_group_norm_dev: activation %d", act);
     PSGPU_REQUIRE(std::isfinite(eps) && eps >= 0.0f, "psgpu_group_norm_dev: eps %g", (double)eps);
     if (total_frames == 0 || n_utt == 0) return PSGPU_OK;
     PSGPU_REQUIRE(x_dev && y_dev && utt_off_dev, "psgpu_group_norm_dev: NULL device buffer");
-    const size_t es = net_dtype_size(dtype);
-    PSGPU_REQUIRE((x_dev == y_dev && x_stride == y_stride)
-                  || net_disjoint(x_dev, net_span(total_frames, x_stride, n_chan, es), y_dev, net_span(total_frames, y_stride, n_chan, es)),
+    const size_t es = net_dtype_size(dtype), need = psgpu_group_norm_work_bytes(n_utt, total_frames, n_groups);
+    const size_t nx = net_span(total_frames, x_stride, n_chan, es), ny = net_span(total_frames, y_stride, n_chan, es);
+    PSGPU_REQUIRE((x_dev == y_dev && x_stride == y_stride) || net_disjoint(x_dev, nx, y_dev, ny),
                   "psgpu_group_norm_dev: the output overlaps the input without being it");
-    PSGPU_REQUIRE(work_bytes >= psgpu_group_norm_work_bytes(n_utt, total_frames, n_groups) && (work_dev || !psgpu_group_norm_work_bytes(n_utt, total_frames, n_groups)),
-                  "psgpu_group_norm_dev: %zu bytes of workspace, psgpu_group_norm_work_bytes asks for %zu", work_bytes,
-                  psgpu_group_norm_work_bytes(n_utt, total_frames, n_groups));
+    PSGPU_REQUIRE(work_bytes >= need && work_dev, "psgpu_group_norm_dev: %zu bytes of workspace, psgpu_group_norm_work_bytes asks for %zu", work_bytes, need);
+    PSGPU_REQUIRE(((uintptr_t)work_dev & 15) == 0, "psgpu_group_norm_dev: the workspace is not aligned to 16 bytes");
+    PSGPU_REQUIRE(net_disjoint(x_dev, nx, work_dev, need) && net_disjoint(y_dev, ny, work_dev, need), "psgpu_group_norm_dev: the workspace overlaps the input or the output");
     const int rc = net_check_device(nullptr);
     if (rc != PSGPU_OK) return rc;
-    const dim3 grid((uint32_t)n_groups, (uint32_t)n_utt);
+    gn_args a = {};
+    a.x = x_dev; a.xs = x_stride; a.off = utt_off_dev; a.n_utt = n_utt; a.total = total_frames; a.n_chan = n_chan; a.per = n_chan / n_groups;
+    a.n_groups = n_groups; a.weight = weight_dev; a.bias = bias_dev; a.eps = eps; a.y = y_dev; a.ys = y_stride; a.part = (double2 *)work_dev;
     const hipStream_t st = (hipStream_t)stream;
-    const int per = n_chan / n_groups;
-    if (dtype == PSGPU_DT_F32)
-        gnorm_group_kernel<float><<<grid, kGnThreads, 0, st>>>((const float *)x_dev, x_stride, utt_off_dev, total_frames, n_chan, per, weight_dev, bias_dev, eps, act, (float *)y_dev, y_stride);
-    else if (dtype == PSGPU_DT_F16)
-        gnorm_group_kernel<psg_half><<<grid, kGnThreads, 0, st>>>((const psg_half *)x_dev, x_stride, utt_off_dev, total_frames, n_chan, per, weight_dev, bias_dev, eps, act, (psg_half *)y_dev, y_stride);
-    else
-        gnorm_group_kernel<psg_bf16><<<grid, kGnThreads, 0, st>>>((const psg_bf16 *)x_dev, x_stride, utt_off_dev, total_frames, n_chan, per, weight_dev, bias_dev, eps, act, (psg_bf16 *)y_dev, y_stride);
+    if (dtype == PSGPU_DT_F32) gn_run_act<float>(a, act, st);
+    else if (dtype == PSGPU_DT_F16) gn_run_act<psg_half>(a, act, st);
+    else gn_run_act<psg_bf16>(a, act, st);
     PSGPU_HIP(hipGetLastError());
     return PSGPU_OK;
 }

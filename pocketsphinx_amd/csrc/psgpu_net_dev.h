@@ -19,6 +19,19 @@ template <> __device__ __forceinline__ psg_bf16 net_cast<psg_bf16>(float v) { re
 // N consecutive elements that need no alignment beyond their own: the hardware serves wide loads and stores at any element address
 template <typename T, int N> struct __attribute__((packed, aligned(sizeof(T)))) net_pack { T v[N]; };
 
+// element e of 16 bytes in four registers (e a constant after unrolling)
+typedef uint32_t net_u32x4 __attribute__((ext_vector_type(4)));
+template <typename T>
+__device__ __forceinline__ float net_elem(const net_u32x4 &v, int e)
+{
+    if constexpr (sizeof(T) == 4) return __uint_as_float(v[e]);
+    else {
+        const uint32_t w = v[e >> 1];
+        if constexpr (__is_same(T, psg_bf16)) return __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
+        else return (float)__builtin_bit_cast(_Float16, (uint16_t)(e & 1 ? w >> 16 : w));
+    }
+}
+
 // The utterance of each of 64 packed rows, row0 + lane: the u with off[u] <= row < off[u + 1], or -1 (in front of the first, behind
 // the last).  Empty utterances are stepped over.  Offsets that do not ascend give some u or -1, never an access outside
 // off[0 .. n_utt].  All lanes of the wavefront call it.  64 offsets a step for the first row (two dependent loads for 4096 utterances;

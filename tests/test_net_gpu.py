@@ -327,6 +327,11 @@ GN = [
     ([300], 2048, 16, "silu", 1e-5),
     ([1200, 1], 1030, 5, "gelu", 0.0),
     ([7, 2], 5000, 1, "none", 1e-5),
+    ([40, 30, 2], 6000, 1, "silu", 1e-5),
+    ([40, 0, 30, 2], 12002, 2, "gelu", 1e-5),
+    ([3300, 1, 700, 0, 45, 2, 90, 1300, 30, 31, 32, 33, 34, 64, 65, 129], 1024, 32, "gelu", 1e-5),
+    ([129, 130, 400, 1] * 2, 2048, 64, "relu", 1e-5),
+    ([2, 0, 5, 1, 9] * 60, 301, 43, "silu", 1e-5),
 ]
 
 
@@ -366,6 +371,27 @@ def test_group_norm_strides_and_alignment(lens, pad, shift, dtype):
     _close(out, want, err, DT[dtype], "y")
     if pad:
         assert torch.equal(torch.nan_to_num(wide[:, 104:]), torch.nan_to_num(keep)), "elements behind a row were written"
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_group_norm_rows_far_apart(dtype):
+    g = torch.Generator().manual_seed(21)
+    off = [0, 3, 20]
+    x = _rand(g, 20, 64, dtype=DT[dtype])
+    want, err = net_ref.gnorm(x, off, 4, None, None, float(np.float32(1e-5)), "gelu")
+    out = _strided(torch.full((20, 64), 7.0, dtype=DT[dtype]), 70001)
+    group_norm(_strided(x, 65536), _dev(off), 4, act="gelu", out=out)
+    _close(out, want, err, DT[dtype], "y")
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_group_norm_activations_over_their_range(act):
+    """values from -40 to 40 through the activation: a group of two far values keeps the others' places (bias alone moves them)"""
+    x = torch.tensor([[1.0, -1.0]]).repeat(4001, 1)
+    b = torch.linspace(-40, 40, 4001)
+    y = torch.cat([group_norm(x[:1].cuda(), _dev([0, 1]), 1, torch.zeros(2, device="cuda"), torch.tensor([float(v), float(v)], device="cuda"), act=act) for v in b[::40]])
+    want = net_ref.act(act, b[::40].double())
+    _close(y[:, 0], want, 9 * net_ref.U * b[::40].double().abs(), torch.float32, act)
 
 
 def test_group_norm_leaves_rows_of_no_utterance():
