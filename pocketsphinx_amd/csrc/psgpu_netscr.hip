@@ -12,12 +12,30 @@
 #include <atomic>
 #include <cmath>
 
+// Memory bounds it: a row is read once, kept in registers, and its scores are written; 64-bit arithmetic is spent on few elements.
 constexpr int kScrThreads = 256;
 
+// one score in 64 bits
+__device__ __forceinline__ int scr_exact(double l, double top, double unit)
+{
+    if (l == top && l != -INFINITY) return 0;
+    if (l != l) return 32767;
+    const double d = floor((top - l) * unit + 0.5);
+    return d < 32767.0 ? (int)d : 32767;
+}
+
+// a difference in 64 bits, where it is needed: the compiler is kept from taking it (or the prior's widening) for every element beforehand
+__device__ __forceinline__ double scr_diff(float z, float p)
+{
+    asm volatile("" : "+v"(z), "+v"(p));
+    return (double)z - (double)p;
+}
+
+// rows longer than the registers: read three times
 template <typename T>
 __global__ __launch_bounds__(kScrThreads)
-void netscr_row_kernel(const T *__restrict__ z, int64_t z_stride, int32_t n_sen, const float *__restrict__ prior, double unit,
-                       int16_t *__restrict__ out, int64_t out_stride, float *__restrict__ best)
+void netscr_long_kernel(const T *__restrict__ z, int64_t z_stride, int32_t n_sen, const float *__restrict__ prior, double unit,
+                        int16_t *__restrict__ out, int64_t out_stride, float *__restrict__ best)
 {
     __shared__ double s_l[kScrThreads / 64];
     __shared__ float s_z[kScrThreads / 64];
@@ -41,14 +59,7 @@ void netscr_row_kernel(const T *__restrict__ z, int64_t z_stride, int32_t n_sen,
     for (int w = 0; w < kScrThreads / 64; ++w) { ml = fmax(ml, s_l[w]); mz = fmaxf(mz, s_z[w]); }
     double sum = 0.0;
     for (int s = tid; s < n_sen; s += kScrThreads) {
-        const double l = like(s);
-        int q = 32767;
-        if (l == ml && l != -INFINITY) q = 0;
-        else if (l == l) {
-            const double d = floor((ml - l) * unit + 0.5);
-            if (d < 32767.0) q = (int)d;
-        }
-        out[t * out_stride + s] = (int16_t)q;
+        out[t * out_stride + s] = (int16_t)scr_exact(like(s), ml, unit);
         sum += (double)expf(net_f32(row[s]) - mz);
     }
     if (!best) return;
@@ -60,6 +71,166 @@ void netscr_row_kernel(const T *__restrict__ z, int64_t z_stride, int32_t n_sen,
         for (int w = 0; w < kScrThreads / 64; ++w) sum += s_sum[w];
         best[t] = nan ? NAN : (mz == -INFINITY ? -INFINITY : (float)(ml - ((double)mz + log(sum))));
     }
+}
+
+// numbers in the order of unsigned integers; not for NaN
+__device__ __forceinline__ unsigned long long scr_key(double v)
+{
+    const unsigned long long b = (unsigned long long)__double_as_longlong(v);
+    return b >> 63 ? ~b : b | 1ull << 63;
+}
+__device__ __forceinline__ double scr_value(unsigned long long k) { return __longlong_as_double((long long)(k >> 63 ? k ^ 1ull << 63 : ~k)); }
+
+// A row a workgroup, NCH chunks of 16 bytes a work-item, in registers; the priors are fetched once for all of a workgroup's rows.
+//
+// l in 32 bits, lf = fl(z - prior), keeps the order: the best l is among those whose lf is the greatest, and only those are taken in 64
+// bits.  A score's q = (top - l) unit + 1/2 in 32 bits is off by at most c + 6 q 2^-23, c = (2 |top| unit + 4) 2^-23: the three
+// differences round by 2^-24 of |top|, |l| <= |top| + (top - l) and top - l, the products and sums by 2^-24 of q each, and twice all that is
+// allowed.  Where q less that and q plus that have one floor it is the score's; else the score is taken in 64 bits (2 in 10000 of
+// a network's outputs).  A NaN and a masked senone end at 32767 by the minimum.  `plain` says that unit is not so far from 1 that these
+// steps leave float's range; without it, or with a best that is not finite, all scores are taken in 64 bits.
+template <typename T, int NT, int NCH>
+__global__ __launch_bounds__(NT, 4)
+void netscr_row_kernel(const T *__restrict__ z, int64_t z_stride, int32_t rows, int32_t n_sen, const float *__restrict__ prior, double unit,
+                       int plain, int16_t *__restrict__ out, int64_t out_stride, float *__restrict__ best)
+{
+    constexpr int E = 16 / sizeof(T), W = NT / 64;
+    constexpr uint32_t kMask = sizeof(T) == 4 ? 0xff800000u : __is_same(T, psg_half) ? 0xfc00fc00u : 0xff80ff80u;      // minus infinity
+    __shared__ float s_l[2][W], s_z[2][W];
+    __shared__ double s_sum[2][W];
+    __shared__ unsigned long long s_top[2];
+    const int tid = threadIdx.x, wave = tid >> 6;
+    const float unitf = (float)unit;
+    float pr[NCH][E];
+#pragma unroll
+    for (int i = 0; i < NCH; ++i)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int s = (i * NT + tid) * E + e;
+            pr[i][e] = prior && s < n_sen ? prior[s] : 0.0f;
+        }
+    int par = 0;
+    for (int64_t t = blockIdx.x; t < rows; t += gridDim.x, par ^= 1) {
+        const T *row = z + t * z_stride;
+        net_u32x4 v[NCH];
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int s = (i * NT + tid) * E;
+            v[i] = net_u32x4{kMask, kMask, kMask, kMask};
+            if (s + E <= n_sen) v[i] = __builtin_bit_cast(net_u32x4, *(const net_pack<T, E> *)(row + s));
+            else if (s < n_sen) {                           // the places behind the row's end are masked
+                net_pack<T, E> w = __builtin_bit_cast(net_pack<T, E>, v[i]);
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (s + e < n_sen) w.v[e] = row[s + e];
+                v[i] = __builtin_bit_cast(net_u32x4, w);
+            }
+        }
+        if (tid == 0) s_top[par] = scr_key(-INFINITY);
+        float ml = -INFINITY, mz = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            asm volatile("" : "+v"(v[i]));                  // (kept as they lie in memory, unpacked where they are used)
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float ze = net_elem<T>(v[i], e);
+                ml = fmaxf(ml, ze - pr[i][e]);              // (fmaxf steps over a NaN)
+                mz = fmaxf(mz, ze);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        for (int o = 32; o; o >>= 1) { ml = fmaxf(ml, __shfl_xor(ml, o)); mz = fmaxf(mz, __shfl_xor(mz, o)); }
+        if ((tid & 63) == 0) { s_l[par][wave] = ml; s_z[par][wave] = mz; }
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < W; ++w) { ml = fmaxf(ml, s_l[par][w]); mz = fmaxf(mz, s_z[par][w]); }
+        float sum = 0.0f;
+        double mine = -INFINITY;
+        bool hit = false;
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            asm volatile("" : "+v"(v[i]));
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float ze = net_elem<T>(v[i], e);
+                if (ze - pr[i][e] == ml) { hit = true; mine = fmax(mine, scr_diff(ze, pr[i][e])); }
+                if (best) sum += __builtin_amdgcn_exp2f((ze - mz) * 1.4426950408889634f);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (hit) atomicMax(&s_top[par], scr_key(mine));
+        double total = sum;
+        if (best) {
+            for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o);
+            if ((tid & 63) == 0) s_sum[par][wave] = total;
+        }
+        __syncthreads();
+        const double top = scr_value(s_top[par]);
+        if (best && tid == 0) {
+            total = 0.0;
+            for (int w = 0; w < W; ++w) total += s_sum[par][w];
+            if (mz > -INFINITY) best[t] = (float)(top - ((double)mz + log(total)));       // (a NaN among the outputs is one in the sum)
+            else {
+                bool nan = false;
+                for (int s = 0; s < n_sen; ++s) { const float ze = net_f32(row[s]); nan |= ze != ze; }
+                best[t] = nan ? NAN : -INFINITY;
+            }
+        }
+        const float topf = ml, c = __builtin_fmaf(fabsf(topf) * 2.0f, unitf, 4.0f) * 0x1p-23f;
+        const bool far = !plain || !(fabsf(topf) < INFINITY);
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int s = (i * NT + tid) * E;
+            asm volatile("" : "+v"(v[i]));
+            __builtin_amdgcn_sched_barrier(0);
+            if (s >= n_sen) continue;
+            int q[E];
+            bool unsure[E], any = false;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float qf = __builtin_fmaf(topf - (net_elem<T>(v[i], e) - pr[i][e]), unitf, 0.5f);
+                const float lo = fminf(floorf(__builtin_fmaf(qf, 1.0f - 6 * 0x1p-23f, -c)), 32767.0f);
+                const float hi = fminf(floorf(__builtin_fmaf(qf, 1.0f + 6 * 0x1p-23f, c)), 32767.0f);
+                q[e] = (int)lo;
+                unsure[e] = far || lo != hi;
+                any |= unsure[e];
+            }
+            if (any)
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (unsure[e]) q[e] = scr_exact(scr_diff(net_elem<T>(v[i], e), pr[i][e]), top, unit);
+            net_pack<int16_t, E> o;
+#pragma unroll
+            for (int e = 0; e < E; ++e) o.v[e] = (int16_t)q[e];
+            int16_t *to = out + t * out_stride + s;
+            if (s + E <= n_sen) *(net_pack<int16_t, E> *)to = o;
+            else
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (s + e < n_sen) to[e] = o.v[e];
+        }
+    }
+}
+
+template <typename T>
+static void scr_run(const void *z, int64_t zs, int32_t rows, int32_t n_sen, const float *prior, double unit, int16_t *out, int64_t os, float *best, hipStream_t st)
+{
+    constexpr int E = 16 / sizeof(T);
+    const int plain = unit >= 1e-6 && unit <= 1e6;
+    const int64_t chunks = ((int64_t)n_sen + E - 1) / E;
+    // up to 8 workgroups a compute unit, each with its share of the rows; few rows: all of a compute unit's wavefronts on each
+#define ROWS(NT, NCH) netscr_row_kernel<T, NT, NCH><<<(uint32_t)(rows < 2048 ? rows : 2048), NT, 0, st>>>((const T *)z, zs, rows, n_sen, prior, unit, plain, out, os, best)
+    if (rows > 512 && chunks <= 256 * 4) {
+        if (chunks <= 256) ROWS(256, 1);
+        else if (chunks <= 256 * 2) ROWS(256, 2);
+        else if (chunks <= 256 * 3) ROWS(256, 3);
+        else ROWS(256, 4);
+    } else if (chunks <= 1024) ROWS(1024, 1);
+    else if (chunks <= 1024 * 2) ROWS(1024, 2);
+    else if (chunks <= 1024 * 3) ROWS(1024, 3);
+    else if (chunks <= 1024 * 5) ROWS(1024, 5);
+    else netscr_long_kernel<T><<<(uint32_t)rows, kScrThreads, 0, st>>>((const T *)z, zs, n_sen, prior, unit, out, os, best);
+#undef ROWS
 }
 
 // hipGetDeviceProperties costs more than a launch: its answer for a device is kept
@@ -95,14 +266,12 @@ extern "C" int psgpu_senone_scores_dev(int32_t dtype, const void *logits_dev, in
     const int rc = net_check_device(nullptr);
     if (rc != PSGPU_OK) return rc;
     const double unit = scale / (std::log(logbase) * (double)(1 << kSenscrShift));
-    const dim3 grid((uint32_t)total_frames);
     const hipStream_t st = (hipStream_t)stream;
-    if (dtype == PSGPU_DT_F32)
-        netscr_row_kernel<float><<<grid, kScrThreads, 0, st>>>((const float *)logits_dev, logits_stride, n_sen, log_prior_dev, unit, senscr_dev, senscr_stride, best_dev);
-    else if (dtype == PSGPU_DT_F16)
-        netscr_row_kernel<psg_half><<<grid, kScrThreads, 0, st>>>((const psg_half *)logits_dev, logits_stride, n_sen, log_prior_dev, unit, senscr_dev, senscr_stride, best_dev);
-    else
-        netscr_row_kernel<psg_bf16><<<grid, kScrThreads, 0, st>>>((const psg_bf16 *)logits_dev, logits_stride, n_sen, log_prior_dev, unit, senscr_dev, senscr_stride, best_dev);
+#define RUN(T) scr_run<T>(logits_dev, logits_stride, total_frames, n_sen, log_prior_dev, unit, senscr_dev, senscr_stride, best_dev, st)
+    if (dtype == PSGPU_DT_F32) RUN(float);
+    else if (dtype == PSGPU_DT_F16) RUN(psg_half);
+    else RUN(psg_bf16);
+#undef RUN
     PSGPU_HIP(hipGetLastError());
     return PSGPU_OK;
 }
