@@ -16,38 +16,67 @@ from . import capi
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 
 
+_DTYPES = {}
+
+
 def _dtypes():
-    import torch
-    return {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    if not _DTYPES:
+        import torch
+        _DTYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+    return _DTYPES
+
+
+class _On:
+    """the device current in a scope, for calls that are made where it is already; gives torch's current stream there, as a handle"""
+    __slots__ = ("index", "back")
+
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self):
+        import torch
+        self.back = torch.cuda.current_device()
+        if self.back != self.index:
+            torch.cuda.set_device(self.index)
+        try:
+            return torch._C._cuda_getCurrentRawStream(self.index)      # (a third of a small call's time less than the stream object)
+        except AttributeError:
+            return torch.cuda.current_stream(self.index).cuda_stream
+
+    def __exit__(self, *exc):
+        if self.back != self.index:
+            import torch
+            torch.cuda.set_device(self.back)
 
 
 def _rows(t, name, width=None, dtype=None, device=None, rows=None):
     """checks a 2-d device tensor of rows; returns its row stride in elements"""
     import torch
-    if not torch.is_tensor(t) or t.dim() != 2:
+    if not isinstance(t, torch.Tensor) or t.dim() != 2:
         raise ValueError("%s: a tensor [frames][width] is needed" % name)
-    if t.device.type != "cuda" or (device is not None and t.device != device):
+    if not t.is_cuda or (device is not None and t.device != device):
         raise ValueError("%s is on %s, not on %s" % (name, t.device, device if device is not None else "a GPU"))
     if dtype is not None and t.dtype != dtype:
         raise ValueError("%s has type %s, not %s" % (name, t.dtype, dtype))
-    if width is not None and t.shape[1] != width:
-        raise ValueError("%s has rows of %d, not of %d" % (name, t.shape[1], width))
-    if rows is not None and t.shape[0] != rows:
-        raise ValueError("%s has %d rows, not %d" % (name, t.shape[0], rows))
-    if t.shape[0] > 0x7fffffff:
-        raise ValueError("%s has %d rows" % (name, t.shape[0]))
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    (n, w), (stride, step) = t.shape, t.stride()
+    if width is not None and w != width:
+        raise ValueError("%s has rows of %d, not of %d" % (name, w, width))
+    if rows is not None and n != rows:
+        raise ValueError("%s has %d rows, not %d" % (name, n, rows))
+    if n > 0x7fffffff:
+        raise ValueError("%s has %d rows" % (name, n))
+    if w > 1 and step != 1:
         raise ValueError("%s: a row's elements must lie side by side" % name)
-    if t.shape[0] <= 1:
-        return max(int(t.shape[1]), 1)
-    if t.stride(0) < t.shape[1]:
+    if n <= 1:
+        return max(w, 1)
+    if stride < w:
         raise ValueError("%s: rows overlap" % name)
-    return int(t.stride(0))
+    return stride
 
 
 def _vector(t, name, n, dtype, device):
     import torch
-    if not torch.is_tensor(t) or t.dim() != 1 or t.dtype != dtype or t.device != device or (n is not None and t.shape[0] != n):
+    if not isinstance(t, torch.Tensor) or t.dim() != 1 or t.dtype != dtype or t.device != device or (n is not None and t.shape[0] != n):
         raise ValueError("%s: a tensor %s of %s on %s is needed" % (name, "[%d]" % n if n is not None else "[n]", dtype, device))
     return t.contiguous()
 
@@ -61,7 +90,7 @@ def _offsets(utt_off, device):
 
 
 def _p(t):
-    return C.c_void_p(None if t is None else t.data_ptr())
+    return None if t is None else t.data_ptr()
 
 
 def _matrix(w, shape_name, dtype=None):
@@ -115,7 +144,7 @@ class AdaptedProjection:
         adapter: int32 [n_utt], each utterance's slot (-1: none)."""
         import torch
         xs = _rows(x, "x", self.d_in, self.dtype, self.device)
-        rows, n_utt = int(x.shape[0]), 0
+        rows, n_utt = x.shape[0], 0
         if utt_off is not None:
             utt_off, n_utt = _offsets(utt_off, self.device)
         if adapter is not None:
@@ -126,14 +155,14 @@ class AdaptedProjection:
         if dt not in (self.dtype, torch.float32) or (out is not None and out_dtype is not None and out_dtype != dt):
             raise ValueError("the output is of the layer's type or float32")
         L = capi.lib()
-        with torch.cuda.device(self.device):
+        with _On(self.device) as stream:
             if out is None:
-                out = torch.empty((rows, self.d_out), dtype=dt, device=self.device)
+                out = x.new_empty((rows, self.d_out), dtype=dt)
             ys = _rows(out, "out", self.d_out, dt, self.device, rows)
             need = int(L.psgpu_proj_work_bytes(self.h, rows)) if utt_off is not None else 0
-            work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+            work = x.new_empty(need, dtype=torch.uint8) if need else None
             capi.check(L.psgpu_proj_run_dev(self.h, _p(x), xs, _p(utt_off), _p(adapter), n_utt, rows, _p(out), ys, _dtypes()[dt], _p(work),
-                                            need, C.c_void_p(torch.cuda.current_stream().cuda_stream)), "psgpu_proj_run_dev")
+                                            need, stream), "psgpu_proj_run_dev")
         return out
 
     def close(self):
@@ -157,20 +186,19 @@ def group_norm(x, utt_off, n_groups, weight=None, bias=None, eps=1e-5, act="none
         raise ValueError("x has type %s" % x.dtype)
     if act not in ACTIVATIONS:
         raise ValueError("act: one of %s" % ", ".join(ACTIVATIONS))
-    rows, chan, dev = int(x.shape[0]), int(x.shape[1]), x.device
+    (rows, chan), dev = x.shape, x.device
     utt_off, n_utt = _offsets(utt_off, dev)
     weight = None if weight is None else _vector(weight, "weight", chan, torch.float32, dev)
     bias = None if bias is None else _vector(bias, "bias", chan, torch.float32, dev)
     L = capi.lib()
-    with torch.cuda.device(dev):
+    with _On(dev) as stream:
         if out is None:
-            out = torch.empty((rows, chan), dtype=x.dtype, device=dev)
+            out = x.new_empty((rows, chan))
         ys = _rows(out, "out", chan, x.dtype, dev, rows)
         need = int(L.psgpu_group_norm_work_bytes(n_utt, rows, int(n_groups)))
-        work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        work = x.new_empty(need, dtype=torch.uint8) if need else None
         capi.check(L.psgpu_group_norm_dev(_dtypes()[x.dtype], _p(x), xs, _p(utt_off), n_utt, rows, chan, int(n_groups), _p(weight), _p(bias),
-                                          float(eps), ACTIVATIONS[act], _p(out), ys, _p(work), need,
-                                          C.c_void_p(torch.cuda.current_stream().cuda_stream)), "psgpu_group_norm_dev")
+                                          float(eps), ACTIVATIONS[act], _p(out), ys, _p(work), need, stream), "psgpu_group_norm_dev")
     return out
 
 
@@ -182,14 +210,13 @@ def senone_scores(logits, log_prior=None, scale=1.0, logbase=1.0001, out=None, w
     zs = _rows(logits, "logits")
     if logits.dtype not in _dtypes():
         raise ValueError("logits have type %s" % logits.dtype)
-    rows, n_sen, dev = int(logits.shape[0]), int(logits.shape[1]), logits.device
+    (rows, n_sen), dev = logits.shape, logits.device
     log_prior = None if log_prior is None else _vector(log_prior, "log_prior", n_sen, torch.float32, dev)
-    with torch.cuda.device(dev):
+    with _On(dev) as stream:
         if out is None:
-            out = torch.empty((rows, n_sen), dtype=torch.int16, device=dev)
+            out = logits.new_empty((rows, n_sen), dtype=torch.int16)
         ss = _rows(out, "out", n_sen, torch.int16, dev, rows)
-        best = torch.empty(rows, dtype=torch.float32, device=dev) if want_best else None
+        best = logits.new_empty(rows, dtype=torch.float32) if want_best else None
         capi.check(capi.lib().psgpu_senone_scores_dev(_dtypes()[logits.dtype], _p(logits), zs, rows, n_sen, _p(log_prior), float(scale),
-                                                      float(logbase), _p(out), ss, _p(best),
-                                                      C.c_void_p(torch.cuda.current_stream().cuda_stream)), "psgpu_senone_scores_dev")
+                                                      float(logbase), _p(out), ss, _p(best), stream), "psgpu_senone_scores_dev")
     return (out, best) if want_best else out
