@@ -69,9 +69,14 @@ __device__ __forceinline__ int net_utt_of_rows(const int32_t *off, int n_utt, in
     return u >= 0 && u < n_utt && off[u] <= row && off[u + 1] > row ? u : -1;
 }
 
-// Waits for this wavefront's loads (vmcnt 0, the other counters left alone).  Loads that go to LDS without a register need it in front of
-// the barrier that hands them to other wavefronts: the barrier's own wait covers LDS instructions, not always these.
-__device__ __forceinline__ void net_wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+// A barrier in front of which this wavefront waits for all of its loads (and stores) but the N issued last, and for its LDS
+// instructions.  Loads that go to LDS without a register need their own wait: a plain barrier's covers LDS instructions, not always these.
+template <int N>
+__device__ __forceinline__ void net_wait_barrier()
+{
+    static_assert(N >= 0 && N < 64, "a counter of six bits");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "i"(N) : "memory");
+}
 
 // ---- matrix instructions ------------------------------------------------------------------------------------------------------------
 // Products of 16 x 16 from 16 bytes a lane: lane l of the first operand holds row l & 15, of the second column l & 15, elements

@@ -11,8 +11,8 @@
 //   W   [outs / 64][chunks][4][64 lanes][16 bytes]          a chunk: KC = 64 bytes of d_in
 //   A   [slot][chunks][ranks / 16][64 lanes][16 bytes]
 //   B   [slot][parts][outs / 64][ranks / KC][4][64 lanes][16 bytes]
-// zeros in the padding.  Fragment f of 64 outputs holds in row m the output (m / 4) * 16 + f * 4 + m % 4: the four fragments leave a
-// lane 16 neighbouring outputs of one frame, 128 bytes a frame in a store.
+// zeros in the padding.  The outputs are dealt to the rows of four fragments so that one store of a wavefront writes 64 neighbouring
+// bytes of each of 16 frames (proj_out_of).
 //
 // The adapters' h is kept in 32 bits, for the half types as two bfloat16 parts (their sum is h to 2^-17) that go through the matrix
 // instructions as one more piece of the reduced axis, against B in bfloat16: float16's B is two parts (exact), of whose products the
@@ -48,7 +48,12 @@ template <typename T> struct proj_b_type { typedef psg_bf16 type; static constex
 template <> struct proj_b_type<float> { typedef float type; static constexpr int parts = 1; };
 template <> struct proj_b_type<psg_half> { typedef psg_bf16 type; static constexpr int parts = 2; };
 
-__device__ __forceinline__ int proj_out_of(int f, int m) { return (m >> 2) * 16 + f * 4 + (m & 3); }
+// the output of 64 that row m of fragment f holds: a lane's four rows m = 4 q .. 4 q + 3 of a fragment (of two, for halves) are 16 bytes
+template <typename T>
+__device__ __forceinline__ int proj_out_of(int f, int m)
+{
+    return sizeof(T) == 4 ? f * 16 + m : (f >> 1) * 32 + (m >> 2) * 8 + (f & 1) * 4 + (m & 3);
+}
 
 // the two bfloat16 parts of a value (an infinity has a second part of 0)
 __device__ __forceinline__ void proj_split(float v, psg_bf16 &hi, psg_bf16 &lo)
@@ -67,7 +72,7 @@ void proj_lay_w_kernel(const T *__restrict__ src, int32_t rows, int32_t cols, in
     const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= n) return;
     const int lane = i & 63, f = (i >> 6) & 3, c = (int)((i >> 8) % chunks);
-    const int o = (int)((i >> 8) / chunks) * 64 + proj_out_of(f, lane & 15), k = c * KC + (lane >> 4) * E;
+    const int o = (int)((i >> 8) / chunks) * 64 + proj_out_of<T>(f, lane & 15), k = c * KC + (lane >> 4) * E;
 #pragma unroll
     for (int e = 0; e < E; ++e) dst[i * E + e] = o < rows && k + e < cols ? src[(size_t)o * cols + k + e] : T{};
 }
@@ -93,7 +98,7 @@ void proj_lay_b_kernel(const T *__restrict__ src, int32_t d_out, int32_t rank, i
     const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= n) return;
     const int lane = i & 63, f = (i >> 6) & 3, c = (int)((i >> 8) % rank_chunks);
-    const int o = (int)((i >> 8) / rank_chunks) * 64 + proj_out_of(f, lane & 15), r = c * KC + (lane >> 4) * E;
+    const int o = (int)((i >> 8) / rank_chunks) * 64 + proj_out_of<T>(f, lane & 15), r = c * KC + (lane >> 4) * E;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         const T v = o < d_out && r + e < rank ? src[(size_t)o * rank + r + e] : T{};
@@ -265,22 +270,24 @@ __device__ __forceinline__ void proj_expand(net_f32x4 (&acc)[MF][NF], int m0, in
 typedef const __attribute__((address_space(1))) uint32_t *net_global_word;
 typedef __attribute__((address_space(3))) uint32_t *net_lds_word;
 
-// A tile of BM = WM MF 16 frames x BN = WN 64 outputs a workgroup; a wavefront MF 16 x 64.  Two stages in LDS of 128 bytes of the
-// reduced axis; while one is multiplied the next is on its way.  x lies in rows of 128 bytes whose 16-byte pieces are exchanged by the
-// row's low bits (piece p of row r holds p ^ (r & 7)), so that 16 rows at once meet no bank twice; W lies as in memory.
+// A tile of BM = WM MF 16 frames x BN = WN 64 outputs a workgroup; a wavefront MF 16 x 64.  A ring of three stages in LDS of 64 bytes
+// of the reduced axis: while one is multiplied the next is there or nearly and the one behind it is on its way.  x lies in rows of 64
+// bytes whose 16-byte pieces are exchanged by the row (piece p of row r at p ^ (r / 2 & 3)), so that 8 lanes meet no bank twice; W
+// lies as in memory.  Two workgroups a compute unit: one's first loads and last stores pass under the other's products (with one of
+// 256 x 256 they cost 18 us a tile, as much as 600 inputs' products).
 // DMA: x is aligned to 16 bytes and goes to LDS without a register.  A last stage that d_in does not fill goes through registers.
 template <typename T, typename Y, bool DMA, int WM, int WN, int MF>
-__global__ __launch_bounds__(WM * WN * 64)
+__global__ __launch_bounds__(WM * WN * 64, 2)
 void proj_tile_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, int32_t d_in, int32_t chunks, const char *__restrict__ w,
                       const float *__restrict__ bias, int32_t d_out, const char *__restrict__ b, size_t b_slot, size_t b_part, int32_t rp,
                       const int32_t *__restrict__ rank, const int32_t *__restrict__ row_slot, const char *__restrict__ h,
                       Y *__restrict__ y, int64_t y_stride, int32_t tiles_m, int32_t tiles_n)
 {
-    constexpr int E = proj_geo<T>::E, KC = proj_geo<T>::KC, W = WM * WN, BM = WM * MF * 16, XB = BM * 128, WB = WN * 8192, ST = XB + WB;
-    constexpr int XI = BM / 8 / W, WI = WN * 8 / W;         // 1 KB pieces of a stage a wavefront
-    static_assert(XI * W * 8 == BM && WI * W == WN * 8, "a stage is shared evenly");
+    constexpr int E = proj_geo<T>::E, KC = proj_geo<T>::KC, W = WM * WN, BM = WM * MF * 16, XB = BM * 64, WB = WN * 4096, ST = XB + WB;
+    constexpr int XI = BM / 16 / W, WI = WN * 4 / W;        // 1 KB pieces of a stage a wavefront
+    static_assert(XI * W * 16 == BM && WI * W == WN * 4, "a stage is shared evenly");
     typedef typename proj_geo<T>::frag frag;
-    __shared__ __attribute__((aligned(1024))) char s_buf[2 * ST];
+    __shared__ __attribute__((aligned(1024))) char s_buf[3 * ST];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
 
     // neighbouring tiles on one die (workgroups are dealt to the 8 dies in turn), 8 rows of tiles deep: they share x and W in its L2
@@ -291,29 +298,29 @@ void proj_tile_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, i
     const int g0 = (in / deep) * WN;                        // first group of 64 outputs
 
     // where this lane's pieces come from: x at a 32-bit offset from the tile's first row (DMA; the host sees to that), W one offset for all
-    const int xk = ((lane & 7) ^ (lane >> 3)) * E;          // element of the stage (rows of a piece start at a multiple of 8)
+    const int xk = ((lane & 3) ^ (lane >> 3 & 3)) * E;      // element of the stage (rows of a piece start at a multiple of 16)
     const char *xt = (const char *)(x + m0 * x_stride);
     const char *wt = w + (size_t)g0 * chunks * 4096;
     typedef typename std::conditional<DMA, uint32_t, uint64_t>::type offs;
     offs xo[XI];
 #pragma unroll
     for (int i = 0; i < XI; ++i) {
-        const int64_t r = min((int64_t)(wave * XI + i) * 8 + (lane >> 3), (int64_t)rows - 1 - m0);
+        const int64_t r = min((int64_t)(wave * XI + i) * 16 + (lane >> 2), (int64_t)rows - 1 - m0);
         xo[i] = (offs)((r * x_stride + xk) * (int64_t)sizeof(T));
     }
-    const int stages = chunks / 2;
-    const int full = d_in / (2 * KC);                       // stages that d_in fills: stages or stages - 1
+    const int full = d_in / KC;                             // stages that d_in fills
+    const int stages = (d_in + KC - 1) / KC;
 
     frag xr[DMA ? 1 : XI];
     auto fetch = [&](int st, int buf) {
         char *to = s_buf + buf * ST;
 #pragma unroll
         for (int i = 0; i < WI; ++i) {
-            const int q = wave * WI + i;                    // [group][8 KB]
-            const char *from = wt + ((size_t)(q >> 3) * chunks * 4096 + (size_t)st * 8192 + (q & 7) * 1024);
+            const int q = wave * WI + i;                    // [group][4 KB]
+            const char *from = wt + ((size_t)(q >> 2) * chunks + st) * 4096 + (q & 3) * 1024;
             __builtin_amdgcn_global_load_lds((net_global_word)(from + (uint32_t)lane * 16), (net_lds_word)(to + XB + q * 1024), 16, 0, 0);
         }
-        const char *from = xt + (size_t)st * 128;
+        const char *from = xt + (size_t)st * 64;
         if (st < full) {
 #pragma unroll
             for (int i = 0; i < XI; ++i) {
@@ -323,8 +330,8 @@ void proj_tile_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, i
         } else {
 #pragma unroll 1
             for (int i = 0; i < XI; ++i) {                  // once a tile
-                const int64_t r = min((int64_t)(wave * XI + i) * 8 + (lane >> 3), (int64_t)rows - 1 - m0);
-                *(frag *)(to + (wave * XI + i) * 1024 + lane * 16) = net_load_chunk(x + (m0 + r) * x_stride, st * 2 * KC + xk, d_in);
+                const int64_t r = min((int64_t)(wave * XI + i) * 16 + (lane >> 2), (int64_t)rows - 1 - m0);
+                *(frag *)(to + (wave * XI + i) * 1024 + lane * 16) = net_load_chunk(x + (m0 + r) * x_stride, st * KC + xk, d_in);
             }
         }
     };
@@ -339,28 +346,33 @@ void proj_tile_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, i
     net_f32x4 acc[MF][4] = {};
     fetch(0, 0);
     put(0, 0);
+    if (stages > 1) {
+        fetch(1, 1);
+        put(1, 1);
+    }
+    int buf = 0;                                            // st % 3
     for (int st = 0; st < stages; ++st) {
-        net_wait_loads();                                   // this wavefront's pieces of the stage lie in LDS; the barrier: everybody's
-        __syncthreads();
-        const int buf = st & 1;
-        if (st + 1 < stages) fetch(st + 1, buf ^ 1);
+        // this wavefront's pieces of stage st lie in LDS (the XI + WI loads of stage st + 1, issued behind them, may be on their way),
+        // its reads of stage st - 1 are done; behind the barrier: everybody's
+        if (st + 1 < stages) net_wait_barrier<XI + WI>();
+        else net_wait_barrier<0>();
+        const int ahead = buf == 0 ? 2 : buf - 1;           // (st + 2) % 3
+        if (st + 2 < stages) fetch(st + 2, ahead);
         const char *from = s_buf + buf * ST;
+        frag wf[4], xf[MF];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            frag wf[4], xf[MF];
+        for (int f = 0; f < 4; ++f) wf[f] = *(const frag *)(from + XB + wn * 4096 + f * 1024 + lane * 16);
 #pragma unroll
-            for (int f = 0; f < 4; ++f) wf[f] = *(const frag *)(from + XB + wn * 8192 + (c * 4 + f) * 1024 + lane * 16);
-#pragma unroll
-            for (int m = 0; m < MF; ++m) {
-                const int r = (wm * MF + m) * 16 + (lane & 15);
-                xf[m] = *(const frag *)(from + r * 128 + (((c * 4 + (lane >> 4)) ^ (r & 7)) * 16));
-            }
-#pragma unroll
-            for (int m = 0; m < MF; ++m)
-#pragma unroll
-                for (int f = 0; f < 4; ++f) acc[m][f] = net_mfma(wf[f], xf[m], acc[m][f]);
+        for (int m = 0; m < MF; ++m) {
+            const int r = (wm * MF + m) * 16 + (lane & 15);
+            xf[m] = *(const frag *)(from + r * 64 + (((lane >> 4) ^ (r >> 1 & 3)) * 16));
         }
-        if (st + 1 < stages) put(st + 1, buf ^ 1);
+#pragma unroll
+        for (int m = 0; m < MF; ++m)
+#pragma unroll
+            for (int f = 0; f < 4; ++f) acc[m][f] = net_mfma(wf[f], xf[m], acc[m][f]);
+        if (st + 2 < stages) put(st + 2, ahead);
+        buf = buf == 2 ? 0 : buf + 1;
     }
 
     int64_t t[MF];
@@ -390,25 +402,29 @@ void proj_tile_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, i
         }
     }
 
-    const int o = (g0 + wn) * 64 + (lane >> 4) * 16;        // this lane's 16 outputs
-    float bo[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) bo[i] = bias[o + i];
     constexpr int SE = 16 / sizeof(Y);
+    int o[4];                                               // this lane's outputs, four a fragment
+    float bo[4][4];
+#pragma unroll
+    for (int f = 0; f < 4; ++f) {
+        o[f] = (g0 + wn) * 64 + proj_out_of<T>(f, (lane >> 4) * 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bo[f][j] = bias[o[f] + j];
+    }
 #pragma unroll
     for (int m = 0; m < MF; ++m) {
         if (slot[m] == kProjNoRow) continue;
-        Y *yr = y + t[m] * y_stride + o;
+        Y *yr = y + t[m] * y_stride;
 #pragma unroll
-        for (int i = 0; i < 16; i += SE) {
+        for (int f = 0; f < 4; f += SE / 4) {
             net_pack<Y, SE> v;
 #pragma unroll
-            for (int j = 0; j < SE; ++j) v.v[j] = net_cast<Y>(acc[m][(i + j) >> 2][(i + j) & 3] + bo[i + j]);
-            if (o + i + SE <= d_out) *(net_pack<Y, SE> *)(yr + i) = v;
+            for (int j = 0; j < SE; ++j) v.v[j] = net_cast<Y>(acc[m][f + (j >> 2)][j & 3] + bo[f + (j >> 2)][j & 3]);
+            if (o[f] + SE <= d_out) *(net_pack<Y, SE> *)(yr + o[f]) = v;
             else
 #pragma unroll
                 for (int j = 0; j < SE; ++j)
-                    if (o + i + j < d_out) yr[i + j] = v.v[j];
+                    if (o[f] + j < d_out) yr[o[f] + j] = v.v[j];
         }
     }
 }
@@ -457,7 +473,7 @@ void proj_few_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, in
         const int m = q / NF, f = q % NF;
         const int64_t t = m0 + m * 16 + (lane & 15);
         const int slot = t >= rows ? kProjNoRow : row_slot ? row_slot[t] : -1;
-        const int ol = (lane >> 4) * 16 + (f0 + f) * 4, o = g * 64 + ol;
+        const int o = g * 64 + proj_out_of<T>(f0 + f, (lane >> 4) * 4);
         net_f32x4 v = s_part[0][q][lane];
         for (int i = 1; i < NW; ++i) v += s_part[i][q][lane];
         if (slot >= 0 && b) {
@@ -662,7 +678,7 @@ static void proj_launch(const psgpu_proj_t *p, const void *x, int64_t xs, const 
     const char *b = adapter ? p->b : nullptr;
     const size_t b_part = p->b_slot / proj_b_type<T>::parts;
     const bool dma = (((uintptr_t)x | (uintptr_t)(xs * sizeof(T))) & 15) == 0 && xs < ((int64_t)1 << 30) / 256 / (int64_t)sizeof(T);
-    const int64_t t128 = (((int64_t)total + 127) / 128) * ((p->d_out + 127) / 128), t256 = (((int64_t)total + 255) / 256) * ((p->d_out + 255) / 256);
+    const int64_t t128 = (((int64_t)total + 127) / 128) * ((p->d_out + 127) / 128), t256 = (((int64_t)total + 255) / 256) * ((p->d_out + 127) / 128);
 #define TILE(D, WM, WN, MF) do { \
         const int32_t tm = (int32_t)(((int64_t)total + WM * MF * 16 - 1) / (WM * MF * 16)), tn = (p->d_out + WN * 64 - 1) / (WN * 64); \
         proj_tile_kernel<T, Y, D, WM, WN, MF><<<(uint32_t)tm * (uint32_t)tn, WM * WN * 64, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, p->w, p->bias, p->d_out, \
@@ -676,10 +692,10 @@ static void proj_launch(const psgpu_proj_t *p, const void *x, int64_t xs, const 
             const dim3 grid((uint32_t)((p->d_out + 63) / 64), (uint32_t)((total + 31) / 32));
             proj_few_kernel<T, Y, 4, 2, 4><<<grid, 256, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, p->w, p->bias, p->d_out, b, p->b_slot, b_part, p->rp, p->rank, slots, h, (Y *)y, ys);
         }
-    } else if (sizeof(T) == 4 || t256 < 512) {
+    } else if (sizeof(T) == 4 || t256 < 1024) {
         if (dma) TILE(true, 2, 2, 4); else TILE(false, 2, 2, 4);
     } else {
-        if constexpr (sizeof(T) == 2) { if (dma) TILE(true, 2, 4, 8); else TILE(false, 2, 4, 8); }
+        if constexpr (sizeof(T) == 2) { if (dma) TILE(true, 2, 2, 8); else TILE(false, 2, 2, 8); }
     }
 #undef TILE
 }
