@@ -31,6 +31,8 @@ __device__ __forceinline__ double scr_diff(float z, float p)
     return (double)z - (double)p;
 }
 
+typedef short scr_short2 __attribute__((ext_vector_type(2)));
+
 // rows longer than the registers: read three times
 template <typename T>
 __global__ __launch_bounds__(kScrThreads)
@@ -86,9 +88,13 @@ __device__ __forceinline__ double scr_value(unsigned long long k) { return __lon
 // l in 32 bits, lf = fl(z - prior), keeps the order: the best l is among those whose lf is the greatest, and only those are taken in 64
 // bits.  A score's q = (top - l) unit + 1/2 in 32 bits is off by at most c + 6 q 2^-23, c = (2 |top| unit + 4) 2^-23: the three
 // differences round by 2^-24 of |top|, |l| <= |top| + (top - l) and top - l, the products and sums by 2^-24 of q each, and twice all that is
-// allowed.  Where q less that and q plus that have one floor it is the score's; else the score is taken in 64 bits (2 in 10000 of
-// a network's outputs).  A NaN and a masked senone end at 32767 by the minimum.  `plain` says that unit is not so far from 1 that these
-// steps leave float's range; without it, or with a best that is not finite, all scores are taken in 64 bits.
+// allowed.  Where q less that and q plus that have one whole part it is the score's; else the score is taken in 64 bits (2 in 10000
+// of a network's outputs).  The conversion to 16 bits ends at 32767, where a NaN and a masked senone are taken too (a minimum steps
+// over a NaN).  `plain` says that unit is not so far from 1 that these steps leave float's range; without it, or with a best that is
+// not finite, all scores are taken in 64 bits.
+//
+// The softmax's sum: exp(z - m) = 2^(z a - m a) in one fused step, a = log2(e) in 32 bits; m a rounded is b, which all terms share, and
+// the logarithm gets b - m a back in 64 bits.
 template <typename T, int NT, int NCH>
 __global__ __launch_bounds__(NT, 4)
 void netscr_row_kernel(const T *__restrict__ z, int64_t z_stride, int32_t rows, int32_t n_sen, const float *__restrict__ prior, double unit,
@@ -131,6 +137,7 @@ void netscr_row_kernel(const T *__restrict__ z, int64_t z_stride, int32_t rows, 
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
             asm volatile("" : "+v"(v[i]));                  // (kept as they lie in memory, unpacked where they are used)
+            if ((i * NT + wave * 64) * E >= n_sen) break;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const float ze = net_elem<T>(v[i], e);
@@ -139,28 +146,43 @@ void netscr_row_kernel(const T *__restrict__ z, int64_t z_stride, int32_t rows, 
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+        const float own = ml;
         for (int o = 32; o; o >>= 1) { ml = fmaxf(ml, __shfl_xor(ml, o)); mz = fmaxf(mz, __shfl_xor(mz, o)); }
         if ((tid & 63) == 0) { s_l[par][wave] = ml; s_z[par][wave] = mz; }
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < W; ++w) { ml = fmaxf(ml, s_l[par][w]); mz = fmaxf(mz, s_z[par][w]); }
-        float sum = 0.0f;
-        double mine = -INFINITY;
-        bool hit = false;
+        if (own == ml) {                                    // the best may be here
+            double mine = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            asm volatile("" : "+v"(v[i]));
+            for (int i = 0; i < NCH; ++i) {
+                asm volatile("" : "+v"(v[i]));
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const float ze = net_elem<T>(v[i], e);
-                if (ze - pr[i][e] == ml) { hit = true; mine = fmax(mine, scr_diff(ze, pr[i][e])); }
-                if (best) sum += __builtin_amdgcn_exp2f((ze - mz) * 1.4426950408889634f);
+                for (int e = 0; e < E; ++e) {
+                    const float ze = net_elem<T>(v[i], e);
+                    if (ze - pr[i][e] == ml) mine = fmax(mine, scr_diff(ze, pr[i][e]));
+                }
             }
-            __builtin_amdgcn_sched_barrier(0);
+            atomicMax(&s_top[par], scr_key(mine));
         }
-        if (hit) atomicMax(&s_top[par], scr_key(mine));
-        double total = sum;
+        const float a = 1.4426950408889634f;
+        const bool huge = !(fabsf(mz) < 1e38f);             // m a could leave float's range; values that far apart are equal or e^-(1e30)
+        const float b = huge ? 0.0f : mz * a;
+        double total = 0.0;
         if (best) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NCH; ++i) {
+                asm volatile("" : "+v"(v[i]));
+                if ((i * NT + wave * 64) * E >= n_sen) break;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float ze = net_elem<T>(v[i], e);
+                    sum += huge ? (ze == mz ? 1.0f : ze != ze ? ze : 0.0f) : __builtin_amdgcn_exp2f(__builtin_fmaf(ze, a, -b));
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            total = sum;
             for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o);
             if ((tid & 63) == 0) s_sum[par][wave] = total;
         }
@@ -169,7 +191,8 @@ void netscr_row_kernel(const T *__restrict__ z, int64_t z_stride, int32_t rows, 
         if (best && tid == 0) {
             total = 0.0;
             for (int w = 0; w < W; ++w) total += s_sum[par][w];
-            if (mz > -INFINITY) best[t] = (float)(top - ((double)mz + log(total)));       // (a NaN among the outputs is one in the sum)
+            if (mz > -INFINITY)                             // (a NaN among the outputs is one in the sum)
+                best[t] = (float)(top - ((double)mz + (log(total) + (huge ? 0.0 : (double)b - (double)mz * (double)a) * 0.69314718055994531)));
             else {
                 bool nan = false;
                 for (int s = 0; s < n_sen; ++s) { const float ze = net_f32(row[s]); nan |= ze != ze; }
@@ -177,28 +200,31 @@ void netscr_row_kernel(const T *__restrict__ z, int64_t z_stride, int32_t rows, 
             }
         }
         const float topf = ml, c = __builtin_fmaf(fabsf(topf) * 2.0f, unitf, 4.0f) * 0x1p-23f;
+        const float unit0 = unitf * (1.0f - 6 * 0x1p-23f), unit1 = unitf * (1.0f + 6 * 0x1p-23f), half0 = 0.5f - c, half1 = 0.5f + c;
         const bool far = !plain || !(fabsf(topf) < INFINITY);
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
             const int s = (i * NT + tid) * E;
             asm volatile("" : "+v"(v[i]));
             __builtin_amdgcn_sched_barrier(0);
-            if (s >= n_sen) continue;
-            int q[E];
-            bool unsure[E], any = false;
+            if (s >= n_sen) break;
+            scr_short2 lo[E / 2];
+            bool unsure[E / 2], any = false;
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const float qf = __builtin_fmaf(topf - (net_elem<T>(v[i], e) - pr[i][e]), unitf, 0.5f);
-                const float lo = fminf(floorf(__builtin_fmaf(qf, 1.0f - 6 * 0x1p-23f, -c)), 32767.0f);
-                const float hi = fminf(floorf(__builtin_fmaf(qf, 1.0f + 6 * 0x1p-23f, c)), 32767.0f);
-                q[e] = (int)lo;
-                unsure[e] = far || lo != hi;
-                any |= unsure[e];
+            for (int e = 0; e < E; e += 2) {
+                const float d0 = fminf(topf - (net_elem<T>(v[i], e) - pr[i][e]), 3e38f), d1 = fminf(topf - (net_elem<T>(v[i], e + 1) - pr[i][e + 1]), 3e38f);
+                lo[e / 2] = __builtin_amdgcn_cvt_pk_i16((int)__builtin_fmaf(d0, unit0, half0), (int)__builtin_fmaf(d1, unit0, half0));
+                const scr_short2 hi = __builtin_amdgcn_cvt_pk_i16((int)__builtin_fmaf(d0, unit1, half1), (int)__builtin_fmaf(d1, unit1, half1));
+                unsure[e / 2] = far || __builtin_bit_cast(uint32_t, lo[e / 2]) != __builtin_bit_cast(uint32_t, hi);
+                any |= unsure[e / 2];
             }
+            int q[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) q[e] = lo[e / 2][e & 1];
             if (any)
 #pragma unroll
                 for (int e = 0; e < E; ++e)
-                    if (unsure[e]) q[e] = scr_exact(scr_diff(net_elem<T>(v[i], e), pr[i][e]), top, unit);
+                    if (unsure[e / 2]) q[e] = scr_exact(scr_diff(net_elem<T>(v[i], e), pr[i][e]), top, unit);
             net_pack<int16_t, E> o;
 #pragma unroll
             for (int e = 0; e < E; ++e) o.v[e] = (int16_t)q[e];

@@ -138,8 +138,9 @@ __device__ __forceinline__ void proj_store_h(net_f32x4 v, float scale, char *h, 
     }
 }
 
-// Many rows: 32 a wavefront, all of an adapter's ranks at once, x once from memory (that is what bounds it), A from the caches.
-template <typename T, int RF>
+// Many rows: MR 16 a wavefront, all of an adapter's ranks at once, x once from memory (that is what bounds it), A from the caches (as
+// many bytes as x with 32 rows and 32 ranks: 64 rows where that leaves enough wavefronts).
+template <typename T, int RF, int MR>
 __global__ __launch_bounds__(256)
 void proj_shrink_kernel(const T *__restrict__ x, int64_t x_stride, int32_t total, int32_t d_in, int32_t chunks, const char *__restrict__ a, size_t a_slot,
                         int32_t rp, const int32_t *__restrict__ rank, const float *__restrict__ scale, int32_t max_adapters,
@@ -149,34 +150,38 @@ void proj_shrink_kernel(const T *__restrict__ x, int64_t x_stride, int32_t total
     constexpr int E = proj_geo<T>::E, KC = proj_geo<T>::KC;
     typedef typename proj_geo<T>::frag frag;
     const int lane = threadIdx.x & 63;
-    const int64_t row0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 32;
+    const int64_t row0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * (MR * 16);
     if (row0 >= total) return;
     const int slot = proj_slot_of_rows(utt_off, adapter, n_utt, rank, max_adapters, (int)row0, total);
-    if (lane < 32 && row0 + lane < total) row_slot[row0 + lane] = slot;
+    if (lane < MR * 16 && row0 + lane < total) row_slot[row0 + lane] = slot;
     if (!a) return;
     const int rank_frags = rp / 16;
-    const T *x0 = x + min(row0 + (lane & 15), (int64_t)total - 1) * x_stride, *x1 = x + min(row0 + 16 + (lane & 15), (int64_t)total - 1) * x_stride;
-    uint64_t todo = __ballot(lane < 32 && slot >= 0);
+    const T *xr[MR];
+#pragma unroll
+    for (int m = 0; m < MR; ++m) xr[m] = x + min(row0 + m * 16 + (lane & 15), (int64_t)total - 1) * x_stride;
+    uint64_t todo = __ballot(lane < MR * 16 && slot >= 0);
     while (todo) {
         const int s = __shfl(slot, __builtin_ctzll(todo));
         const uint64_t mine = __ballot(slot == s);
         todo &= ~mine;
         const frag *as = (const frag *)(a + s * a_slot) + lane;
-        net_f32x4 acc[2][RF] = {};
+        net_f32x4 acc[MR][RF] = {};
 #pragma unroll 2
         for (int c = 0; c < chunks; ++c) {
             const int k = c * KC + (lane >> 4) * E;
-            const frag f0 = net_load_chunk(x0, k, d_in), f1 = net_load_chunk(x1, k, d_in);
+            frag f[MR];
+#pragma unroll
+            for (int m = 0; m < MR; ++m) f[m] = net_load_chunk(xr[m], k, d_in);
 #pragma unroll
             for (int q = 0; q < RF; ++q) {
                 const frag w = as[(c * rank_frags + min(q, rank_frags - 1)) * 64];
-                acc[0][q] = net_mfma(w, f0, acc[0][q]);
-                acc[1][q] = net_mfma(w, f1, acc[1][q]);
+#pragma unroll
+                for (int m = 0; m < MR; ++m) acc[m][q] = net_mfma(w, f[m], acc[m][q]);
             }
         }
         const float sc = scale[s];
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+        for (int m = 0; m < MR; ++m)
             if (mine >> (m * 16 + (lane & 15)) & 1)
 #pragma unroll
                 for (int q = 0; q < RF; ++q)
@@ -232,37 +237,27 @@ void proj_shrink_few_kernel(const T *__restrict__ x, int64_t x_stride, int32_t t
 
 // ---- the product in tiles -----------------------------------------------------------------------------------------------------------
 // acc of 16 frames (column lane & 15) += B_s h over the ranks of adapter s, for the frames whose slot it is
-template <typename T, int NF, int MF>
-__device__ __forceinline__ void proj_expand(net_f32x4 (&acc)[MF][NF], int m0, int m1, const int (&slot)[MF], int s, const char *b, size_t b_slot, size_t b_part, size_t b_group,
-                                            int chunks, int rp, const char *h, const int64_t (&t)[MF])
+template <typename T>
+__device__ __forceinline__ void proj_expand(net_f32x4 (&acc)[4], bool mine, const char *bs, size_t b_part, int chunks, const char *ht, int rp)
 {
     constexpr int E = proj_geo<T>::E, KC = proj_geo<T>::KC;
     typedef typename proj_b_type<T>::type B;
     typedef typename net_frag<B>::type bfrag;
     const int lane = threadIdx.x & 63;
-    const char *bs = b + s * b_slot + b_group;
+#pragma unroll 1
     for (int c = 0; c < chunks; ++c) {
-        bfrag w[NF], w2[NF];
-#pragma unroll
-        for (int f = 0; f < NF; ++f) {
-            w[f] = ((const bfrag *)(bs + (size_t)(f >> 2) * rp * 64 * sizeof(B)))[(c * 4 + (f & 3)) * 64 + lane];
-            if constexpr (proj_b_type<T>::parts == 2) w2[f] = ((const bfrag *)(bs + b_part + (size_t)(f >> 2) * rp * 64 * sizeof(B)))[(c * 4 + (f & 3)) * 64 + lane];
+        bfrag hi = {}, lo = {};
+        if (mine) {
+            const B *hr = (const B *)ht + c * KC + (lane >> 4) * E;
+            hi = *(const bfrag *)hr;
+            if constexpr (proj_geo<T>::parts == 2) lo = *(const bfrag *)(hr + rp);
         }
 #pragma unroll
-        for (int m = 0; m < MF; ++m) {
-            if (m < m0 || m >= m1) continue;
-            bfrag hi = {}, lo = {};
-            if (slot[m] == s) {
-                const B *hr = (const B *)h + (size_t)t[m] * proj_geo<T>::parts * rp + c * KC + (lane >> 4) * E;
-                hi = *(const bfrag *)hr;
-                if constexpr (proj_geo<T>::parts == 2) lo = *(const bfrag *)(hr + rp);
-            }
-#pragma unroll
-            for (int f = 0; f < NF; ++f) {
-                acc[m][f] = net_mfma(w[f], hi, acc[m][f]);
-                if constexpr (proj_geo<T>::parts == 2) acc[m][f] = net_mfma(w[f], lo, acc[m][f]);
-                if constexpr (proj_b_type<T>::parts == 2) acc[m][f] = net_mfma(w2[f], hi, acc[m][f]);
-            }
+        for (int f = 0; f < 4; ++f) {
+            const bfrag w = ((const bfrag *)bs)[(c * 4 + f) * 64 + lane];
+            acc[f] = net_mfma(w, hi, acc[f]);
+            if constexpr (proj_geo<T>::parts == 2) acc[f] = net_mfma(w, lo, acc[f]);
+            if constexpr (proj_b_type<T>::parts == 2) acc[f] = net_mfma(((const bfrag *)(bs + b_part))[(c * 4 + f) * 64 + lane], hi, acc[f]);
         }
     }
 }
@@ -276,6 +271,8 @@ typedef __attribute__((address_space(3))) uint32_t *net_lds_word;
 // lies as in memory.  Two workgroups a compute unit: one's first loads and last stores pass under the other's products (with one of
 // 256 x 256 they cost 18 us a tile, as much as 600 inputs' products).
 // DMA: x is aligned to 16 bytes and goes to LDS without a register.  A last stage that d_in does not fill goes through registers.
+// Where all of a tile's frames have one adapter its h and B are more stages of the same ring (h's parts against B's); else every
+// fragment of frames takes its adapters in turn behind them.
 template <typename T, typename Y, bool DMA, int WM, int WN, int MF>
 __global__ __launch_bounds__(WM * WN * 64, 2)
 void proj_tile_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, int32_t d_in, int32_t chunks, const char *__restrict__ w,
@@ -310,10 +307,28 @@ void proj_tile_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, i
     }
     const int full = d_in / KC;                             // stages that d_in fills
     const int stages = (d_in + KC - 1) / KC;
+    int total = stages, slot0 = -1, rchunks = 0;            // with an adapter's stages
 
     frag xr[DMA ? 1 : XI];
     auto fetch = [&](int st, int buf) {
         char *to = s_buf + buf * ST;
+        if (st >= stages) {                                 // B's parts 0, 0, 1 against h's 0, 1, 0
+            const int part = (st - stages) / rchunks, c = (st - stages) - part * rchunks;
+            const char *bs = b + slot0 * b_slot + (part == 2 ? b_part : 0) + (size_t)g0 * rp * 64 * sizeof(typename proj_b_type<T>::type) + (size_t)c * 4096;
+#pragma unroll
+            for (int i = 0; i < WI; ++i) {
+                const int q = wave * WI + i;
+                const char *from = bs + (size_t)(q >> 2) * rp * 64 * sizeof(typename proj_b_type<T>::type) + (q & 3) * 1024;
+                __builtin_amdgcn_global_load_lds((net_global_word)(from + (uint32_t)lane * 16), (net_lds_word)(to + XB + q * 1024), 16, 0, 0);
+            }
+            const char *hs = h + (size_t)m0 * rp * 4 + (part == 1 ? rp * 2 : 0) + (size_t)c * 64;
+#pragma unroll
+            for (int i = 0; i < XI; ++i) {
+                const int r = (int)min((int64_t)(wave * XI + i) * 16 + (lane >> 2), (int64_t)rows - 1 - m0);
+                __builtin_amdgcn_global_load_lds((net_global_word)(hs + (uint32_t)(r * rp * 4 + xk * (int)sizeof(T))), (net_lds_word)(to + (wave * XI + i) * 1024), 16, 0, 0);
+            }
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < WI; ++i) {
             const int q = wave * WI + i;                    // [group][4 KB]
@@ -350,22 +365,35 @@ void proj_tile_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, i
         fetch(1, 1);
         put(1, 1);
     }
+    bool mixed = false;
+    if (row_slot && b) {
+        slot0 = __builtin_amdgcn_readfirstlane(row_slot[m0]);
+        int same = 1;
+        for (int r = threadIdx.x; r < BM; r += W * 64) same &= row_slot[min(m0 + r, (int64_t)rows - 1)] == slot0;
+        mixed = !__syncthreads_and(same);
+        if (!mixed && slot0 >= 0) {
+            rchunks = (rank[slot0] + KC - 1) / KC;
+            total += rchunks * (sizeof(T) == 4 ? 1 : 1 + proj_b_type<T>::parts);
+        }
+        if (stages == 1 && total > 1) fetch(1, 1);
+    }
     int buf = 0;                                            // st % 3
-    for (int st = 0; st < stages; ++st) {
+    auto step = [&](int st, auto of) {
+        typedef decltype(of) F;
         // this wavefront's pieces of stage st lie in LDS (the XI + WI loads of stage st + 1, issued behind them, may be on their way),
         // its reads of stage st - 1 are done; behind the barrier: everybody's
-        if (st + 1 < stages) net_wait_barrier<XI + WI>();
+        if (st + 1 < total) net_wait_barrier<XI + WI>();
         else net_wait_barrier<0>();
         const int ahead = buf == 0 ? 2 : buf - 1;           // (st + 2) % 3
-        if (st + 2 < stages) fetch(st + 2, ahead);
+        if (st + 2 < total) fetch(st + 2, ahead);
         const char *from = s_buf + buf * ST;
-        frag wf[4], xf[MF];
+        F wf[4], xf[MF];
 #pragma unroll
-        for (int f = 0; f < 4; ++f) wf[f] = *(const frag *)(from + XB + wn * 4096 + f * 1024 + lane * 16);
+        for (int f = 0; f < 4; ++f) wf[f] = *(const F *)(from + XB + wn * 4096 + f * 1024 + lane * 16);
 #pragma unroll
         for (int m = 0; m < MF; ++m) {
             const int r = (wm * MF + m) * 16 + (lane & 15);
-            xf[m] = *(const frag *)(from + r * 64 + (((lane >> 4) ^ (r >> 1 & 3)) * 16));
+            xf[m] = *(const F *)(from + r * 64 + (((lane >> 4) ^ (r >> 1 & 3)) * 16));
         }
 #pragma unroll
         for (int m = 0; m < MF; ++m)
@@ -373,6 +401,13 @@ void proj_tile_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, i
             for (int f = 0; f < 4; ++f) acc[m][f] = net_mfma(wf[f], xf[m], acc[m][f]);
         if (st + 2 < stages) put(st + 2, ahead);
         buf = buf == 2 ? 0 : buf + 1;
+    };
+    typedef typename net_frag<typename proj_b_type<T>::type>::type bfrag;
+    if constexpr (std::is_same<frag, bfrag>::value)
+        for (int st = 0; st < total; ++st) step(st, frag());
+    else {
+        for (int st = 0; st < stages; ++st) step(st, frag());
+        for (int st = stages; st < total; ++st) step(st, bfrag());
     }
 
     int64_t t[MF];
@@ -381,23 +416,15 @@ void proj_tile_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, i
     int slot[MF];
 #pragma unroll
     for (int m = 0; m < MF; ++m) slot[m] = t[m] >= rows ? kProjNoRow : row_slot ? row_slot[t[m]] : -1;
-    if (row_slot && b) {
-        const size_t group = (size_t)(g0 + wn) * rp * 64 * sizeof(typename proj_b_type<T>::type);
-        const int s0 = __shfl(slot[0], 0);
-        bool same = true;
+    if (mixed) {
+        const char *bg = b + (size_t)(g0 + wn) * rp * 64 * sizeof(typename proj_b_type<T>::type);
 #pragma unroll
-        for (int m = 0; m < MF; ++m) same &= slot[m] == s0;
-        if (__all(same)) {
-            if (s0 >= 0) proj_expand<T, 4, MF>(acc, 0, MF, slot, s0, b, b_slot, b_part, group, (rank[s0] + KC - 1) / KC, rp, h, t);
-        } else {
-#pragma unroll
-            for (int m = 0; m < MF; ++m) {
-                uint64_t todo = __ballot(slot[m] >= 0);
-                while (todo) {
-                    const int s = __shfl(slot[m], __builtin_ctzll(todo));
-                    todo &= ~__ballot(slot[m] == s);
-                    proj_expand<T, 4, MF>(acc, m, m + 1, slot, s, b, b_slot, b_part, group, (rank[s] + KC - 1) / KC, rp, h, t);
-                }
+        for (int m = 0; m < MF; ++m) {
+            uint64_t todo = __ballot(slot[m] >= 0);
+            while (todo) {
+                const int s = __shfl(slot[m], __builtin_ctzll(todo));
+                todo &= ~__ballot(slot[m] == s);
+                proj_expand<T>(acc[m], slot[m] == s, bg + s * b_slot, b_part, (rank[s] + KC - 1) / KC, h + (size_t)t[m] * rp * 4, rp);
             }
         }
     }
@@ -651,10 +678,12 @@ static void proj_shrink(const psgpu_proj_t *p, const void *x, int64_t xs, const 
     // few rows: one a workgroup up to 2048 of them, so that all run at once
     const bool few = total <= 16384;
     const int32_t tile = total <= 2048 ? 1 : total <= 8192 ? 4 : 16;
-    const uint32_t grid = few ? (uint32_t)((total + tile - 1) / tile) : (uint32_t)(((int64_t)total + 127) / 128);
+    const bool wide = total >= 131072;
+    const uint32_t grid = few ? (uint32_t)((total + tile - 1) / tile) : (uint32_t)(((int64_t)total + (wide ? 255 : 127)) / (wide ? 256 : 128));
 #define SHRINK(RF) do { \
         if (few) proj_shrink_few_kernel<T, RF><<<grid, 256, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, a, p->a_slot, p->rp, p->rank, p->scale, p->max_adapters, off, adapter, n_utt, tile, slots, h); \
-        else proj_shrink_kernel<T, RF><<<grid, 256, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, a, p->a_slot, p->rp, p->rank, p->scale, p->max_adapters, off, adapter, n_utt, slots, h); \
+        else if (wide) proj_shrink_kernel<T, RF, 4><<<grid, 256, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, a, p->a_slot, p->rp, p->rank, p->scale, p->max_adapters, off, adapter, n_utt, slots, h); \
+        else proj_shrink_kernel<T, RF, 2><<<grid, 256, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, a, p->a_slot, p->rp, p->rank, p->scale, p->max_adapters, off, adapter, n_utt, slots, h); \
     } while (0)
     if (p->rp <= 16) SHRINK(1);
     else if (p->rp <= 32) SHRINK(2);
