@@ -254,6 +254,101 @@ void gnorm_held_kernel(gn_args a)
         }
 }
 
+// As above, one group a slice, for slices that fill the registers: workgroups go from one (utterance, group) to the next, and while one's
+// results leave the next one's rows come into the registers that they free.  (Without that a compute unit's two workgroups load,
+// compute and store in step: 634 us for 384 k rows of 1024 in 32 groups.)  Neighbouring groups, which share lines of memory, run on
+// one die (workgroups are dealt to the 8 dies in turn).
+template <typename T, int NT, int NCH, int ACT>
+__global__ __launch_bounds__(NT, 4)
+void gnorm_stream_kernel(gn_args a)
+{
+    constexpr int E = 16 / sizeof(T);
+    __shared__ double2 s_red[NT];
+    __shared__ gn_stat s_stat[1];
+    const T *x = (const T *)a.x;
+    T *y = (T *)a.y;
+    const int64_t items = (int64_t)a.n_utt * a.n_groups;
+    const int cw = a.per / E, nrl = NT / cw, rl = (int)threadIdx.x / cw, ck = (int)threadIdx.x - rl * cw;
+    const uint32_t x_step = (uint32_t)(nrl * (int)a.xs) * sizeof(T), y_step = (uint32_t)(nrl * (int)a.ys) * sizeof(T);
+    const uint32_t x0 = (uint32_t)((rl < nrl ? rl : 0) * (int)a.xs + ck * E) * sizeof(T), y0 = (uint32_t)((rl < nrl ? rl : 0) * (int)a.ys + ck * E) * sizeof(T);
+    // the next item that has rows, from `item` on
+    auto next_of = [&](int64_t item, int &t0, int &len) {
+        for (; item < items; item += gridDim.x) {
+            const int u = (int)(item / a.n_groups);
+            t0 = max(a.off[u], 0);
+            len = min(a.off[u + 1], a.total) - t0;
+            if (len > 0) break;
+        }
+        return item;
+    };
+    int t0 = 0, len = 0;
+    int64_t item = next_of((gridDim.x & 7) == 0 ? (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3) : blockIdx.x, t0, len);
+    if (item >= items) return;
+    net_u32x4 held[NCH];
+    int mine = rl < nrl && rl < len ? (len - 1 - rl) / nrl + 1 : 0;
+    const char *xu = (const char *)(x + t0 * a.xs + (item % a.n_groups) * a.per);
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        held[i] = {};
+        if (i < mine) held[i] = __builtin_bit_cast(net_u32x4, *(const net_pack<T, E> *)(xu + (x0 + i * x_step)));
+    }
+    while (item < items) {
+        const int c = (int)(item % a.n_groups) * a.per + ck * E;
+        double sum[1] = {}, sq[1] = {};
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            gn_add<T, 1>(sum, sq, held[i]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // rows beyond the registers
+#pragma unroll 1
+        for (int i = NCH; i < mine; ++i) gn_add<T, 1>(sum, sq, __builtin_bit_cast(net_u32x4, *(const net_pack<T, E> *)(x + ((int64_t)t0 + rl + (int64_t)i * nrl) * a.xs + c)));
+        double s = sum[0], q = sq[0];
+        gn_sum_lanes(s, q, 64);
+        if ((threadIdx.x & 63) == 0) s_red[threadIdx.x >> 6] = make_double2(s, q);
+        __syncthreads();
+        if (threadIdx.x < 64) {
+            const double2 v = threadIdx.x < NT / 64 ? s_red[threadIdx.x] : make_double2(0.0, 0.0);
+            s = v.x; q = v.y;
+            gn_sum_lanes(s, q, NT / 64);
+            if (threadIdx.x == 0) s_stat[0] = gn_finish(make_double2(s, q), (double)len * a.per, a.eps);
+        }
+        __syncthreads();
+        const gn_stat st = s_stat[0];
+        gn_affine<E> f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            f.mhi[e] = st.mhi;
+            f.mlo[e] = st.mlo;
+            f.rw[e] = a.weight ? st.rstd * a.weight[c + e] : st.rstd;
+            f.b[e] = a.bias ? a.bias[c + e] : 0.0f;
+        }
+        const int was = mine, t_was = t0;
+        char *yu = (char *)(y + t0 * a.ys + (c - ck * E));
+        item = next_of(item + gridDim.x, t0, len);
+        mine = item < items && rl < nrl && rl < len ? (len - 1 - rl) / nrl + 1 : 0;
+        if (item < items) xu = (const char *)(x + t0 * a.xs + (item % a.n_groups) * a.per);
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) asm volatile("" : "+v"(held[i]));
+        uint32_t xo = x0, yo = y0;
+        asm volatile("" : "+v"(xo), "+v"(yo));          // (or all 2 NCH offsets are kept in registers from item to item)
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            if (i < was) gn_store<T, ACT, true>(held[i], f, (T *)(yu + yo), 0, E);
+            held[i] = {};
+            if (i < mine) held[i] = __builtin_bit_cast(net_u32x4, *(const net_pack<T, E> *)(xu + xo));
+            xo += x_step;
+            yo += y_step;
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll 1
+        for (int i = NCH; i < was; ++i) {
+            const int64_t r = (int64_t)t_was + rl + (int64_t)i * nrl;
+            gn_store<T, ACT, true>(__builtin_bit_cast(net_u32x4, *(const net_pack<T, E> *)(x + r * a.xs + c)), f, y + r * a.ys, c, c + E);
+        }
+    }
+}
+
 // ---- tiles of rows, in two passes ----------------------------------------------------------------------------------------------------
 // Rows row .. tile_end - 1 begin in which utterance, and how far it reaches; false: no more utterances in the tile.  Partial sums lie
 // at tile + utterance: along the rows one of the two grows from piece to piece, so every piece has a place of its own.
@@ -380,8 +475,8 @@ static void gn_run(gn_args a, hipStream_t st)
     auto chunks = [&](int64_t g) { return mean_len * ((g * a.per + E - 1) / E); };      // of an utterance's slice of g groups
     auto slices = [&](int64_t g) { return (a.n_groups + g - 1) / g; };
     // One launch where an utterance's group fits a workgroup's registers on average and there are enough of them: 256 work-items hold
-    // 8 chunks each, 512 hold 24.
-    const bool near_rows = a.xs < 1 << 16 && a.ys < 1 << 16;       // 512 x 24 rows of them lie within 2^32 bytes
+    // 8 chunks each, 1024 hold 12.
+    const bool near_rows = a.xs < 1 << 16 && a.ys < 1 << 16;       // 1024 x 12 rows of them lie within 2^32 bytes
     if (near_rows && chunks(1) <= 256 * 8 && ((int64_t)a.total * a.n_chan <= 1 << 17 || (int64_t)a.n_utt * a.n_groups >= 256)) {
         while (gs > 1 && (chunks(gs) > 256 * 8 || a.n_utt * slices(gs) < 512)) gs = (gs + 1) / 2;
         a.gs = (int32_t)gs;
@@ -391,9 +486,9 @@ static void gn_run(gn_args a, hipStream_t st)
         else gnorm_held_kernel<T, 256, 8, E, false, ACT><<<grid, 256, 0, st>>>(a);
         return;
     }
-    if (near_rows && one && chunks(1) <= 512 * 24 && (int64_t)a.n_utt * a.n_groups >= 512) {
+    if (near_rows && one && chunks(1) <= 1024 * 12 && (int64_t)a.n_utt * a.n_groups >= 512) {
         a.gs = 1;
-        gnorm_held_kernel<T, 512, 24, 1, true, ACT><<<dim3((uint32_t)a.n_groups, (uint32_t)a.n_utt), 512, 0, st>>>(a);
+        gnorm_stream_kernel<T, 1024, 12, ACT><<<256, 1024, 0, st>>>(a);              // one workgroup a compute unit
         return;
     }
     a.gs = (int32_t)gs;

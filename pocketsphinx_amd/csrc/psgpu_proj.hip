@@ -717,6 +717,9 @@ static void proj_launch(const psgpu_proj_t *p, const void *x, int64_t xs, const 
         if (total <= 16) {
             const dim3 grid((uint32_t)((p->d_out + 63) / 64 * 4), 1);
             proj_few_kernel<T, Y, 4, 1, 1><<<grid, 256, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, p->w, p->bias, p->d_out, b, p->b_slot, b_part, p->rp, p->rank, slots, h, (Y *)y, ys);
+        } else if ((int64_t)((p->d_out + 63) / 64) * ((total + 31) / 32) < 512) {      // 512 rows to 1024: 19.5 against 20.8 us
+            const dim3 grid((uint32_t)((p->d_out + 63) / 64), (uint32_t)((total + 15) / 16));
+            proj_few_kernel<T, Y, 4, 1, 4><<<grid, 256, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, p->w, p->bias, p->d_out, b, p->b_slot, b_part, p->rp, p->rank, slots, h, (Y *)y, ys);
         } else {
             const dim3 grid((uint32_t)((p->d_out + 63) / 64), (uint32_t)((total + 31) / 32));
             proj_few_kernel<T, Y, 4, 2, 4><<<grid, 256, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, p->w, p->bias, p->d_out, b, p->b_slot, b_part, p->rp, p->rank, slots, h, (Y *)y, ys);
