@@ -486,7 +486,7 @@ static void gn_run(gn_args a, hipStream_t st)
         else gnorm_held_kernel<T, 256, 8, E, false, ACT><<<grid, 256, 0, st>>>(a);
         return;
     }
-    if (near_rows && one && chunks(1) <= 1024 * 12 && (int64_t)a.n_utt * a.n_groups >= 512) {
+    if (near_rows && one && a.per <= 1024 * E && chunks(1) <= 1024 * 12 && (int64_t)a.n_utt * a.n_groups >= 512) {
         a.gs = 1;
         gnorm_stream_kernel<T, 1024, 12, ACT><<<256, 1024, 0, st>>>(a);              // one workgroup a compute unit
         return;

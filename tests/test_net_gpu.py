@@ -332,6 +332,8 @@ GN = [
     ([3300, 1, 700, 0, 45, 2, 90, 1300, 30, 31, 32, 33, 34, 64, 65, 129], 1024, 32, "gelu", 1e-5),
     ([129, 130, 400, 1] * 2, 2048, 64, "relu", 1e-5),
     ([2, 0, 5, 1, 9] * 60, 301, 43, "silu", 1e-5),
+    ([1] * 512, 17000, 1, "none", 1e-5),
+    ([3000, 0, 1, 2, 70, 13000], 512, 128, "silu", 1e-5),
 ]
 
 
@@ -371,6 +373,19 @@ def test_group_norm_strides_and_alignment(lens, pad, shift, dtype):
     _close(out, want, err, DT[dtype], "y")
     if pad:
         assert torch.equal(torch.nan_to_num(wide[:, 104:]), torch.nan_to_num(keep)), "elements behind a row were written"
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_tensors_that_ask_for_a_gradient_are_refused(dtype):
+    x = torch.zeros(6, 12, dtype=DT[dtype], device="cuda", requires_grad=True)
+    w = torch.zeros(12, device="cuda", requires_grad=True)
+    layer = AdaptedProjection(torch.zeros(8, 12, dtype=DT[dtype], requires_grad=True))
+    off = _dev([0, 6])
+    for call in (lambda: group_norm(x, off, 3), lambda: group_norm(x.detach(), off, 3, w), lambda: senone_scores(x), lambda: layer(x)):
+        with pytest.raises(ValueError):
+            call()
+    with torch.no_grad():
+        assert group_norm(x, off, 3, w).shape == x.shape and senone_scores(x).shape == x.shape and layer(x).shape == (6, 8)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
