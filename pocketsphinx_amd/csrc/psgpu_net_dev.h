@@ -78,6 +78,21 @@ __device__ __forceinline__ void net_wait_barrier()
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "i"(N) : "memory");
 }
 
+// Loads to LDS without a register: `bytes` (16 or 4) a lane from base + off (off the lane's, base all lanes'), to lds + lane * bytes.
+// In assembly, so that the compiler does not know them: it would wait for all of them in front of every read of LDS, also of parts
+// that they do not write (128 k rows of 1024 to 1024 outputs: 695 TFLOP/s that way).  net_wait_barrier() is the wait they need; they have
+// no result in registers, and waits that the compiler places for its own loads only become longer by them.  (The idle cycles: a vector
+// instruction may just have written `base`.)
+template <int bytes>
+__device__ __forceinline__ void net_load_lds(const void *base, uint32_t off, uint32_t lds)
+{
+    static_assert(bytes == 16 || bytes == 4, "a size that the instruction has");
+    if constexpr (bytes == 16) asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(off), "s"(base), "s"(lds) : "memory", "m0");
+    else asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dword %0, %1" :: "v"(off), "s"(base), "s"(lds) : "memory", "m0");
+}
+// where an object in LDS begins
+template <typename T> __device__ __forceinline__ uint32_t net_lds_at(T *p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)p; }
+
 // ---- matrix instructions ------------------------------------------------------------------------------------------------------------
 // Products of 16 x 16 from 16 bytes a lane: lane l of the first operand holds row l & 15, of the second column l & 15, elements
 // (l >> 4) * E .. + E - 1 of the reduced axis (E = 16 bytes of T; one instruction of 4 E elements for halves, four of 4 for floats, which

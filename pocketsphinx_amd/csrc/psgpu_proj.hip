@@ -111,6 +111,9 @@ void proj_lay_b_kernel(const T *__restrict__ src, int32_t d_out, int32_t rank, i
     }
 }
 
+// an adapter that is laid out becomes a slot's
+__global__ void proj_load_kernel(int32_t *rank, float *scale, int32_t slot, int32_t r, float s) { rank[slot] = r; scale[slot] = s; }
+
 // which adapter a row has; the lane's row is row0 + lane, kProjNoRow beyond `total`
 __device__ __forceinline__ int proj_slot_of_rows(const int32_t *utt_off, const int32_t *adapter, int n_utt, const int32_t *rank, int max_adapters, int row0, int total)
 {
@@ -262,18 +265,16 @@ __device__ __forceinline__ void proj_expand(net_f32x4 (&acc)[4], bool mine, cons
     }
 }
 
-typedef const __attribute__((address_space(1))) uint32_t *net_global_word;
-typedef __attribute__((address_space(3))) uint32_t *net_lds_word;
-
 // A tile of BM = WM MF 16 frames x BN = WN 64 outputs a workgroup; a wavefront MF 16 x 64.  A ring of three stages in LDS of 64 bytes
 // of the reduced axis: while one is multiplied the next is there or nearly and the one behind it is on its way.  x lies in rows of 64
 // bytes whose 16-byte pieces are exchanged by the row (piece p of row r at p ^ (r / 2 & 3)), so that 8 lanes meet no bank twice; W
 // lies as in memory.  Two workgroups a compute unit: one's first loads and last stores pass under the other's products (with one of
 // 256 x 256 they cost 18 us a tile, as much as 600 inputs' products).
-// DMA: x is aligned to 16 bytes and goes to LDS without a register.  A last stage that d_in does not fill goes through registers.
+// DMA: x goes to LDS without a register, 16 bytes a lane where it is aligned to them, else 4 bytes (rows of 429 floats: 22 % of the
+// time saved over registers), or 0: through registers.  A last stage that d_in does not fill goes through registers.
 // Where all of a tile's frames have one adapter its h and B are more stages of the same ring (h's parts against B's); else every
 // fragment of frames takes its adapters in turn behind them.
-template <typename T, typename Y, bool DMA, int WM, int WN, int MF>
+template <typename T, typename Y, int DMA, int WM, int WN, int MF>
 __global__ __launch_bounds__(WM * WN * 64, 2)
 void proj_tile_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, int32_t d_in, int32_t chunks, const char *__restrict__ w,
                       const float *__restrict__ bias, int32_t d_out, const char *__restrict__ b, size_t b_slot, size_t b_part, int32_t rp,
@@ -282,6 +283,7 @@ void proj_tile_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, i
 {
     constexpr int E = proj_geo<T>::E, KC = proj_geo<T>::KC, W = WM * WN, BM = WM * MF * 16, XB = BM * 64, WB = WN * 4096, ST = XB + WB;
     constexpr int XI = BM / 16 / W, WI = WN * 4 / W;        // 1 KB pieces of a stage a wavefront
+    constexpr int XP = DMA == 4 ? 4 : 1, XL = XI * XP;      // loads of a piece of x, of all
     static_assert(XI * W * 16 == BM && WI * W == WN * 4, "a stage is shared evenly");
     typedef typename proj_geo<T>::frag frag;
     __shared__ __attribute__((aligned(1024))) char s_buf[3 * ST];
@@ -298,56 +300,58 @@ void proj_tile_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, i
     const int xk = ((lane & 3) ^ (lane >> 3 & 3)) * E;      // element of the stage (rows of a piece start at a multiple of 16)
     const char *xt = (const char *)(x + m0 * x_stride);
     const char *wt = w + (size_t)g0 * chunks * 4096;
-    typedef typename std::conditional<DMA, uint32_t, uint64_t>::type offs;
-    offs xo[XI];
+    typedef typename std::conditional<DMA != 0, uint32_t, uint64_t>::type offs;
+    offs xo[XL];
 #pragma unroll
-    for (int i = 0; i < XI; ++i) {
-        const int64_t r = min((int64_t)(wave * XI + i) * 16 + (lane >> 2), (int64_t)rows - 1 - m0);
-        xo[i] = (offs)((r * x_stride + xk) * (int64_t)sizeof(T));
+    for (int i = 0; i < XL; ++i) {
+        // a load of 4 bytes a lane brings 4 rows: lane = row, piece, word
+        const int in = DMA == 4 ? (i & 3) * 4 + (lane >> 4) : lane >> 2;
+        const int64_t r = min((int64_t)(wave * XI + i / XP) * 16 + in, (int64_t)rows - 1 - m0);
+        xo[i] = (offs)(r * x_stride * (int64_t)sizeof(T) + (DMA == 4 ? ((lane >> 2 & 3) ^ (in >> 1 & 3)) * 16 + (lane & 3) * 4 : xk * (int)sizeof(T)));
     }
     const int full = d_in / KC;                             // stages that d_in fills
     const int stages = (d_in + KC - 1) / KC;
     int total = stages, slot0 = -1, rchunks = 0;            // with an adapter's stages
 
     frag xr[DMA ? 1 : XI];
-    auto fetch = [&](int st, int buf) {
-        char *to = s_buf + buf * ST;
-        if (st >= stages) {                                 // B's parts 0, 0, 1 against h's 0, 1, 0
-            const int part = (st - stages) / rchunks, c = (st - stages) - part * rchunks;
-            const char *bs = b + slot0 * b_slot + (part == 2 ? b_part : 0) + (size_t)g0 * rp * 64 * sizeof(typename proj_b_type<T>::type) + (size_t)c * 4096;
-#pragma unroll
-            for (int i = 0; i < WI; ++i) {
-                const int q = wave * WI + i;
-                const char *from = bs + (size_t)(q >> 2) * rp * 64 * sizeof(typename proj_b_type<T>::type) + (q & 3) * 1024;
-                __builtin_amdgcn_global_load_lds((net_global_word)(from + (uint32_t)lane * 16), (net_lds_word)(to + XB + q * 1024), 16, 0, 0);
-            }
-            const char *hs = h + (size_t)m0 * rp * 4 + (part == 1 ? rp * 2 : 0) + (size_t)c * 64;
-#pragma unroll
-            for (int i = 0; i < XI; ++i) {
-                const int r = (int)min((int64_t)(wave * XI + i) * 16 + (lane >> 2), (int64_t)rows - 1 - m0);
-                __builtin_amdgcn_global_load_lds((net_global_word)(hs + (uint32_t)(r * rp * 4 + xk * (int)sizeof(T))), (net_lds_word)(to + (wave * XI + i) * 1024), 16, 0, 0);
-            }
-            return;
-        }
+    const uint32_t lds = net_lds_at(s_buf);
+    auto fetch_full = [&](int st, int buf) {                // a stage that d_in fills
+        const uint32_t to = lds + buf * ST;
+        const char *ws = wt + (size_t)st * 4096, *from = xt + (size_t)st * 64;
 #pragma unroll
         for (int i = 0; i < WI; ++i) {
             const int q = wave * WI + i;                    // [group][4 KB]
-            const char *from = wt + ((size_t)(q >> 2) * chunks + st) * 4096 + (q & 3) * 1024;
-            __builtin_amdgcn_global_load_lds((net_global_word)(from + (uint32_t)lane * 16), (net_lds_word)(to + XB + q * 1024), 16, 0, 0);
+            net_load_lds<16>(ws + (size_t)(q >> 2) * chunks * 4096 + (q & 3) * 1024, lane * 16, to + XB + q * 1024);
         }
-        const char *from = xt + (size_t)st * 64;
-        if (st < full) {
 #pragma unroll
-            for (int i = 0; i < XI; ++i) {
-                if constexpr (DMA) __builtin_amdgcn_global_load_lds((net_global_word)(from + xo[i]), (net_lds_word)(to + (wave * XI + i) * 1024), 16, 0, 0);
-                else xr[i] = __builtin_bit_cast(frag, *(const net_pack<T, E> *)(from + xo[i]));
-            }
-        } else {
+        for (int i = 0; i < XL; ++i) {
+            if constexpr (DMA == 16) net_load_lds<16>(from, xo[i], to + (wave * XI + i) * 1024);
+            else if constexpr (DMA == 4) net_load_lds<4>(from, xo[i], to + wave * XI * 1024 + i * 256);
+            else xr[i] = __builtin_bit_cast(frag, *(const net_pack<T, E> *)(from + xo[i]));
+        }
+    };
+    auto fetch = [&](int st, int buf) {
+        if (st < full) {
+            fetch_full(st, buf);
+            return;
+        }
+        const uint32_t to = lds + buf * ST;
+        // the last stage of d_in, or an adapter's: B's parts 0, 0, 1 against h's 0, 1, 0
+        const bool own = st < stages;
+        const int part = own ? 0 : (st - stages) / rchunks, c = own ? st : (st - stages) - part * rchunks;
+        const size_t group = own ? (size_t)chunks * 4096 : (size_t)rp * 64 * sizeof(typename proj_b_type<T>::type);
+        const char *ws = (own ? wt : b + slot0 * b_slot + (part == 2 ? b_part : 0) + (size_t)g0 * group) + (size_t)c * 4096;
+#pragma unroll
+        for (int i = 0; i < WI; ++i) {
+            const int q = wave * WI + i;
+            net_load_lds<16>(ws + (size_t)(q >> 2) * group + (q & 3) * 1024, lane * 16, to + XB + q * 1024);
+        }
+        const char *hs = h + (size_t)m0 * rp * 4 + (part == 1 ? rp * 2 : 0) + (size_t)c * 64;
 #pragma unroll 1
-            for (int i = 0; i < XI; ++i) {                  // once a tile
-                const int64_t r = min((int64_t)(wave * XI + i) * 16 + (lane >> 2), (int64_t)rows - 1 - m0);
-                *(frag *)(to + (wave * XI + i) * 1024 + lane * 16) = net_load_chunk(x + (m0 + r) * x_stride, st * KC + xk, d_in);
-            }
+        for (int i = 0; i < XI; ++i) {
+            const int64_t r = min((int64_t)(wave * XI + i) * 16 + (lane >> 2), (int64_t)rows - 1 - m0);
+            if (own) *(frag *)(s_buf + buf * ST + (wave * XI + i) * 1024 + lane * 16) = net_load_chunk(x + (m0 + r) * x_stride, st * KC + xk, d_in);
+            else net_load_lds<16>(hs, (uint32_t)((int)r * rp * 4 + xk * (int)sizeof(T)), to + (wave * XI + i) * 1024);
         }
     };
     auto put = [&](int st, int buf) {                       // the pieces that came through registers
@@ -378,14 +382,16 @@ void proj_tile_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, i
         if (stages == 1 && total > 1) fetch(1, 1);
     }
     int buf = 0;                                            // st % 3
-    auto step = [&](int st, auto of) {
+    auto step = [&](int st, auto of, auto steady) {
         typedef decltype(of) F;
-        // this wavefront's pieces of stage st lie in LDS (the XI + WI loads of stage st + 1, issued behind them, may be on their way),
-        // its reads of stage st - 1 are done; behind the barrier: everybody's
-        if (st + 1 < total) net_wait_barrier<XI + WI>();
+        // this wavefront's pieces of stage st lie in LDS (the loads of stage st + 1, issued behind them, may be on their way: XL + WI,
+        // or XI + WI of an adapter's, or none but W's), its reads of stage st - 1 are done; behind the barrier: everybody's
+        if (steady.value || st + 1 < full) net_wait_barrier<XL + WI>();
+        else if (st + 1 < total) net_wait_barrier<XI + WI>();
         else net_wait_barrier<0>();
         const int ahead = buf == 0 ? 2 : buf - 1;           // (st + 2) % 3
-        if (st + 2 < total) fetch(st + 2, ahead);
+        if (steady.value) fetch_full(st + 2, ahead);
+        else if (st + 2 < total) fetch(st + 2, ahead);
         const char *from = s_buf + buf * ST;
         F wf[4], xf[MF];
 #pragma unroll
@@ -399,15 +405,17 @@ void proj_tile_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, i
         for (int m = 0; m < MF; ++m)
 #pragma unroll
             for (int f = 0; f < 4; ++f) acc[m][f] = net_mfma(wf[f], xf[m], acc[m][f]);
-        if (st + 2 < stages) put(st + 2, ahead);
+        if (steady.value || st + 2 < stages) put(st + 2, ahead);
         buf = buf == 2 ? 0 : buf + 1;
     };
     typedef typename net_frag<typename proj_b_type<T>::type>::type bfrag;
+    int st = 0;
+    for (; st + 2 < full; ++st) step(st, frag(), std::true_type());
     if constexpr (std::is_same<frag, bfrag>::value)
-        for (int st = 0; st < total; ++st) step(st, frag());
+        for (; st < total; ++st) step(st, frag(), std::false_type());
     else {
-        for (int st = 0; st < stages; ++st) step(st, frag());
-        for (int st = stages; st < total; ++st) step(st, bfrag());
+        for (; st < stages; ++st) step(st, frag(), std::false_type());
+        for (; st < total; ++st) step(st, bfrag(), std::false_type());
     }
 
     int64_t t[MF];
@@ -642,17 +650,29 @@ extern "C" int psgpu_proj_set_adapter(psgpu_proj_t *p, int32_t slot, int32_t ran
     PSGPU_REQUIRE(psgpu_get_device() == p->device, "psgpu_proj_set_adapter: the projection lives on device %d, the current one is %d", p->device, psgpu_get_device());
     const size_t es = net_dtype_size(p->dtype), raw_a = (size_t)rank * p->d_in * es, at_b = (raw_a + 15) / 16 * 16;
     PSGPU_HIP(hipDeviceSynchronize());              // calls that read the slot have ended; later ones see it whole
-    const int32_t none = 0;
-    PSGPU_HIP(hipMemcpy(p->rank + slot, &none, 4, hipMemcpyHostToDevice));      // (a copy that fails leaves the slot empty)
-    if (!rank) return PSGPU_OK;
-    PSGPU_HIP(hipMemcpy(p->raw, a, raw_a, hipMemcpyDefault));
-    PSGPU_HIP(hipMemcpy(p->raw + at_b, b, (size_t)rank * p->d_out * es, hipMemcpyDefault));
-    if (p->dtype == PSGPU_DT_F32) proj_lay_ab<float>(p, slot, rank, p->raw, p->raw + at_b);
-    else if (p->dtype == PSGPU_DT_F16) proj_lay_ab<psg_half>(p, slot, rank, p->raw, p->raw + at_b);
-    else proj_lay_ab<psg_bf16>(p, slot, rank, p->raw, p->raw + at_b);
+    proj_load_kernel<<<1, 1>>>(p->rank, p->scale, slot, 0, 0.0f);                   // (a copy that fails leaves the slot empty)
     PSGPU_HIP(hipGetLastError());
-    PSGPU_HIP(hipMemcpy(p->scale + slot, &scale, 4, hipMemcpyHostToDevice));
-    PSGPU_HIP(hipMemcpy(p->rank + slot, &rank, 4, hipMemcpyHostToDevice));
+    if (rank) {
+        auto here = [&](const void *v) {            // in this device's memory, at an address that its type asks for
+            hipPointerAttribute_t at;
+            if (hipPointerGetAttributes(&at, v) != hipSuccess) { (void)hipGetLastError(); return false; }
+            return at.type == hipMemoryTypeDevice && at.device == p->device && ((uintptr_t)v & (es - 1)) == 0;
+        };
+        if (!here(a)) {
+            PSGPU_HIP(hipMemcpy(p->raw, a, raw_a, hipMemcpyDefault));
+            a = p->raw;
+        }
+        if (!here(b)) {
+            PSGPU_HIP(hipMemcpy(p->raw + at_b, b, (size_t)rank * p->d_out * es, hipMemcpyDefault));
+            b = p->raw + at_b;
+        }
+        if (p->dtype == PSGPU_DT_F32) proj_lay_ab<float>(p, slot, rank, (const char *)a, (const char *)b);
+        else if (p->dtype == PSGPU_DT_F16) proj_lay_ab<psg_half>(p, slot, rank, (const char *)a, (const char *)b);
+        else proj_lay_ab<psg_bf16>(p, slot, rank, (const char *)a, (const char *)b);
+        PSGPU_HIP(hipGetLastError());
+        proj_load_kernel<<<1, 1>>>(p->rank, p->scale, slot, rank, scale);
+        PSGPU_HIP(hipGetLastError());
+    }
     PSGPU_HIP(hipDeviceSynchronize());
     return PSGPU_OK;
 }
@@ -706,8 +726,10 @@ static void proj_launch(const psgpu_proj_t *p, const void *x, int64_t xs, const 
     }
     const char *b = adapter ? p->b : nullptr;
     const size_t b_part = p->b_slot / proj_b_type<T>::parts;
-    const bool dma = (((uintptr_t)x | (uintptr_t)(xs * sizeof(T))) & 15) == 0 && xs < ((int64_t)1 << 30) / 256 / (int64_t)sizeof(T);
+    const uintptr_t at = (uintptr_t)x | (uintptr_t)(xs * sizeof(T));
+    const bool near_rows = xs < ((int64_t)1 << 30) / 256 / (int64_t)sizeof(T);      // (a tile's rows at 32-bit offsets)
     const int64_t t128 = (((int64_t)total + 127) / 128) * ((p->d_out + 127) / 128), t256 = (((int64_t)total + 255) / 256) * ((p->d_out + 127) / 128);
+    const int dma = !near_rows ? 0 : (at & 15) == 0 ? 16 : (at & 3) == 0 ? 4 : 0;
 #define TILE(D, WM, WN, MF) do { \
         const int32_t tm = (int32_t)(((int64_t)total + WM * MF * 16 - 1) / (WM * MF * 16)), tn = (p->d_out + WN * 64 - 1) / (WN * 64); \
         proj_tile_kernel<T, Y, D, WM, WN, MF><<<(uint32_t)tm * (uint32_t)tn, WM * WN * 64, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, p->w, p->bias, p->d_out, \
@@ -725,9 +747,9 @@ static void proj_launch(const psgpu_proj_t *p, const void *x, int64_t xs, const 
             proj_few_kernel<T, Y, 4, 2, 4><<<grid, 256, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, p->w, p->bias, p->d_out, b, p->b_slot, b_part, p->rp, p->rank, slots, h, (Y *)y, ys);
         }
     } else if (sizeof(T) == 4 || t256 < 1024) {
-        if (dma) TILE(true, 2, 2, 4); else TILE(false, 2, 2, 4);
+        if (dma == 16) TILE(16, 2, 2, 4); else if (dma == 4) TILE(4, 2, 2, 4); else TILE(0, 2, 2, 4);
     } else {
-        if constexpr (sizeof(T) == 2) { if (dma) TILE(true, 2, 2, 8); else TILE(false, 2, 2, 8); }
+        if constexpr (sizeof(T) == 2) { if (dma == 16) TILE(16, 2, 2, 8); else if (dma == 4) TILE(4, 2, 2, 8); else TILE(0, 2, 2, 8); }
     }
 #undef TILE
 }

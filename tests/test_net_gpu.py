@@ -190,6 +190,8 @@ LARGE = [
     (128, 2100, 2500, 8),
     (136, 5126, 6500, 0),
     (128, 5126, 6500, 1),
+    (136, 5126, 1000, 2),
+    (150, 5126, 6500, 6),
     (24, 8192, 4300, 0),
 ]
 
@@ -216,7 +218,7 @@ def test_projection_in_large_tiles(ci, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("pad", [0, 3])
+@pytest.mark.parametrize("pad", [0, 2, 3])
 @pytest.mark.parametrize("rows, d_in, d_out", [(20000, 1000, 2100), (4300, 1024, 8192), (2500, 2048, 1024)])
 def test_projection_over_many_stages(rows, d_in, d_out, pad, dtype):
     """a long reduced axis in large tiles: every stage is whole before it is multiplied (64-bit products on the device)"""
