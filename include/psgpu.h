@@ -1213,8 +1213,8 @@ int psgpu_proj_run_dev(psgpu_proj_t *p, const void *x_dev, int64_t x_stride, con
 /* y[t][c] = act((x[t][c] - m) / sqrt(v + eps) * weight[c] + bias[c]), m and v the mean and the biased variance of an utterance's frames x
  * the channels of c's group (n_chan / n_groups neighbouring channels): cmn() with -varnorm (cmn.c:166-233) per group, with a learned
  * scale.  weight_dev / bias_dev [n_chan] float or NULL (1 / 0).  y_dev has x_dev's type; it may be x_dev with the same stride, and may
- * not overlap it otherwise.  An utterance of a live stream's step is normalised over that step's frames.  At most 65535 utterances.
- * work_dev: psgpu_group_norm_work_bytes bytes, 16-byte aligned (may be NULL when that is 0). */
+ * not overlap it otherwise.  An utterance of a live stream's step is normalised over that step's frames.  At most 65535 utterances and 2^30
+ * channels.  work_dev: psgpu_group_norm_work_bytes bytes, 16-byte aligned. */
 size_t psgpu_group_norm_work_bytes(int32_t n_utt, int32_t total_frames, int32_t n_groups);
 int psgpu_group_norm_dev(int32_t dtype, const void *x_dev, int64_t x_stride, const int32_t *utt_off_dev, int32_t n_utt,
                          int32_t total_frames, int32_t n_chan, int32_t n_groups, const float *weight_dev, const float *bias_dev,

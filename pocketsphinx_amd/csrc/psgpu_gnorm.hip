@@ -194,7 +194,8 @@ __device__ __forceinline__ void gn_store(const net_u32x4 &v, const gn_affine<16 
 }
 
 // ---- an utterance's slice a workgroup ----------------------------------------------------------------------------------------------
-// The first NCH chunks of a work-item stay in registers from the sums to the result: what fits there is read once.
+// The first NCH chunks of a work-item stay in registers from the sums to the result: what fits there is read once.  512 utterances of
+// 10 frames of 1024: 11 us, one trip to memory, the sums' join and the stores.
 template <typename T, int NT, int NCH, int K, bool FULL, int ACT>
 __global__ __launch_bounds__(NT, 4)
 void gnorm_held_kernel(gn_args a)
@@ -257,7 +258,8 @@ void gnorm_held_kernel(gn_args a)
 // As above, one group a slice, for slices that fill the registers: workgroups go from one (utterance, group) to the next, and while one's
 // results leave the next one's rows come into the registers that they free.  (Without that a compute unit's two workgroups load,
 // compute and store in step: 634 us for 384 k rows of 1024 in 32 groups.)  Neighbouring groups, which share lines of memory, run on
-// one die (workgroups are dealt to the 8 dies in turn).
+// one die (workgroups are dealt to the 8 dies in turn; 577 -> 534 us).  384 k rows of 1024 in 32 groups with GELU: 505 us, 3.1 TB/s; some
+// 360 us of it are vector instructions, 30 a value.
 template <typename T, int NT, int NCH, int ACT>
 __global__ __launch_bounds__(NT, 4)
 void gnorm_stream_kernel(gn_args a)
@@ -349,7 +351,7 @@ void gnorm_stream_kernel(gn_args a)
     }
 }
 
-// ---- tiles of rows, in two passes ----------------------------------------------------------------------------------------------------
+// ---- tiles of rows, in two passes: 102 k rows of 429 floats in 50 + 97 us, 3.5 TB/s ----------------------------------------------------------------------------------------------------
 // Rows row .. tile_end - 1 begin in which utterance, and how far it reaches; false: no more utterances in the tile.  Partial sums lie
 // at tile + utterance: along the rows one of the two grows from piece to piece, so every piece has a place of its own.
 __device__ __forceinline__ bool gn_next(const gn_args &a, int &row, int tile_end, int &u, int &end)

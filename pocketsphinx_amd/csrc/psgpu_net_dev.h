@@ -80,7 +80,7 @@ __device__ __forceinline__ void net_wait_barrier()
 
 // Loads to LDS without a register: `bytes` (16 or 4) a lane from base + off (off the lane's, base all lanes'), to lds + lane * bytes.
 // In assembly, so that the compiler does not know them: it would wait for all of them in front of every read of LDS, also of parts
-// that they do not write (128 k rows of 1024 to 1024 outputs: 695 TFLOP/s that way).  net_wait_barrier() is the wait they need; they have
+// that they do not write (128 k rows of 1024 to 1024 outputs: 725 against 786 TFLOP/s).  net_wait_barrier() is the wait they need; they have
 // no result in registers, and waits that the compiler places for its own loads only become longer by them.  (The idle cycles: a vector
 // instruction may just have written `base`.)
 template <int bytes>
