@@ -207,8 +207,9 @@ void netscr_row_kernel(const T *__restrict__ z, int64_t z_stride, int32_t rows, 
             }
         }
         const float topf = ml, c = __builtin_fmaf(fabsf(topf) * 2.0f, unitf, 4.0f) * 0x1p-23f;
-        const float unit0 = unitf * (1.0f - 6 * 0x1p-23f), unit1 = unitf * (1.0f + 6 * 0x1p-23f), half0 = 0.5f - c, half1 = 0.5f + c;
-        const bool far = !plain || !(fabsf(topf) < INFINITY);
+        const bool far = !plain || !(fabsf(topf) < INFINITY);       // then the two are 0 and -5: unlike everywhere
+        const float unit0 = far ? 0.0f : unitf * (1.0f - 6 * 0x1p-23f), unit1 = far ? 0.0f : unitf * (1.0f + 6 * 0x1p-23f);
+        const float half0 = far ? 0.0f : 0.5f - c, half1 = far ? -5.0f : 0.5f + c;
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
             int me = tid;
@@ -224,7 +225,7 @@ void netscr_row_kernel(const T *__restrict__ z, int64_t z_stride, int32_t rows, 
                 const float d0 = fminf(topf - (net_elem<T>(v[i], e) - pr[i][e]), 3e38f), d1 = fminf(topf - (net_elem<T>(v[i], e + 1) - pr[i][e + 1]), 3e38f);
                 lo[e / 2] = __builtin_amdgcn_cvt_pk_i16((int)__builtin_fmaf(d0, unit0, half0), (int)__builtin_fmaf(d1, unit0, half0));
                 const scr_short2 hi = __builtin_amdgcn_cvt_pk_i16((int)__builtin_fmaf(d0, unit1, half1), (int)__builtin_fmaf(d1, unit1, half1));
-                unsure[e / 2] = far || __builtin_bit_cast(uint32_t, lo[e / 2]) != __builtin_bit_cast(uint32_t, hi);
+                unsure[e / 2] = __builtin_bit_cast(uint32_t, lo[e / 2]) != __builtin_bit_cast(uint32_t, hi);
                 any |= unsure[e / 2];
             }
             int16_t *to = out + t * out_stride + s;

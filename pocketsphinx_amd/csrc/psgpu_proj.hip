@@ -488,6 +488,13 @@ void proj_few_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, in
 #pragma unroll
     for (int m = 0; m < MF; ++m) xp[m] = x + min(m0 + m * 16 + (lane & 15), (int64_t)rows - 1) * x_stride;
     const frag *wp = (const frag *)(w + (size_t)g * chunks * 4096) + f0 * 64 + lane;
+    int slots[MF], ranks[MF];                               // of this lane's frames, asked for in front of the products
+#pragma unroll
+    for (int m = 0; m < MF; ++m) {
+        const int64_t t = m0 + m * 16 + (lane & 15);
+        slots[m] = t >= rows ? kProjNoRow : row_slot ? row_slot[t] : -1;
+        ranks[m] = slots[m] >= 0 && b ? rank[slots[m]] : 0;
+    }
     net_f32x4 acc[MF][NF] = {};
 #pragma unroll 4
     for (int c = wave; c < chunks; c += NW) {
@@ -509,12 +516,15 @@ void proj_few_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, in
     for (int q = wave; q < MF * NF; q += NW) {
         const int m = q / NF, f = q % NF;
         const int64_t t = m0 + m * 16 + (lane & 15);
-        const int slot = t >= rows ? kProjNoRow : row_slot ? row_slot[t] : -1;
+        int slot = slots[0], rank_of = ranks[0];
+#pragma unroll
+        for (int i = 1; i < MF; ++i)
+            if (m == i) { slot = slots[i]; rank_of = ranks[i]; }
         const int o = g * 64 + proj_out_of<T>(f0 + f, (lane >> 4) * 4);
         net_f32x4 v = s_part[0][q][lane];
         for (int i = 1; i < NW; ++i) v += s_part[i][q][lane];
         if (slot >= 0 && b) {
-            const int chunks_r = (rank[slot] + KC - 1) / KC;
+            const int chunks_r = (rank_of + KC - 1) / KC;
             const B *bs = (const B *)(b + slot * b_slot) + (size_t)g * rp * 64 + (f0 + f) * 64 * E;
             const B *hr = (const B *)h + t * proj_geo<T>::parts * rp;
             for (int p = 0; p < chunks_r * 4; ++p) {        // E ranks at a time
