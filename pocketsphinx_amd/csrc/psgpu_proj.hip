@@ -470,17 +470,22 @@ void proj_tile_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, i
 // MF 16 frames x NF 16 outputs a workgroup, whose wavefronts share the reduced axis; no LDS on the way in (nothing is used twice), all of
 // a wavefront's loads on their way at once.  The adapters' terms are taken by the vector units, a lane one frame and four outputs:
 // neighbouring rows seldom share an adapter here.
-template <typename T, typename Y, int NW, int MF, int NF>
+// OWN_H (up to kProjOwnRows rows): every workgroup computes the frames' h for itself, in 32 bits, so that one launch does.
+constexpr int kProjOwnRows = 4;
+template <typename T, typename Y, int NW, int MF, int NF, bool OWN_H>
 __global__ __launch_bounds__(NW * 64)
 void proj_few_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, int32_t d_in, int32_t chunks, const char *__restrict__ w,
                      const float *__restrict__ bias, int32_t d_out, const char *__restrict__ b, size_t b_slot, size_t b_part, int32_t rp,
                      const int32_t *__restrict__ rank, const int32_t *__restrict__ row_slot, const char *__restrict__ h,
-                     Y *__restrict__ y, int64_t y_stride)
+                     Y *__restrict__ y, int64_t y_stride, const char *__restrict__ a, size_t a_slot, const float *__restrict__ scale,
+                     int32_t max_adapters, const int32_t *__restrict__ utt_off, const int32_t *__restrict__ adapter, int32_t n_utt)
 {
     constexpr int E = proj_geo<T>::E, KC = proj_geo<T>::KC;
     typedef typename proj_geo<T>::frag frag;
     typedef typename proj_b_type<T>::type B;
+    static_assert(!OWN_H || MF == 1, "frames of one fragment");
     __shared__ net_f32x4 s_part[NW][MF * NF][64];
+    __shared__ __attribute__((aligned(16))) float s_h[OWN_H ? kProjOwnRows * PSGPU_PROJ_MAX_RANK : 4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t m0 = (int64_t)blockIdx.y * MF * 16;
     const int n0 = blockIdx.x * NF, g = n0 >> 2, f0 = n0 & 3;
@@ -492,7 +497,8 @@ void proj_few_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, in
 #pragma unroll
     for (int m = 0; m < MF; ++m) {
         const int64_t t = m0 + m * 16 + (lane & 15);
-        slots[m] = t >= rows ? kProjNoRow : row_slot ? row_slot[t] : -1;
+        if constexpr (OWN_H) slots[m] = __shfl(proj_slot_of_rows(utt_off, adapter, n_utt, rank, max_adapters, 0, rows), lane & 15);
+        else slots[m] = t >= rows ? kProjNoRow : row_slot ? row_slot[t] : -1;
         ranks[m] = slots[m] >= 0 && b ? rank[slots[m]] : 0;
     }
     net_f32x4 acc[MF][NF] = {};
@@ -512,6 +518,35 @@ void proj_few_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, in
     for (int m = 0; m < MF; ++m)
 #pragma unroll
         for (int f = 0; f < NF; ++f) s_part[wave][m * NF + f][lane] = acc[m][f];
+    if constexpr (OWN_H) {
+        for (int i = threadIdx.x; i < kProjOwnRows * rp; i += NW * 64) s_h[i] = 0.0f;
+        uint64_t todo = __ballot(lane < kProjOwnRows && slots[0] >= 0 && b);    // (the same in all wavefronts)
+        const int rank_frags = rp / 16;
+        __shared__ net_f32x4 s_hp[NW][64];
+        while (todo) {
+            const int s = __shfl(slots[0], __builtin_ctzll(todo));
+            todo &= ~__ballot(slots[0] == s);
+            const frag *as = (const frag *)(a + s * a_slot) + lane;
+            const float sc = scale[s];
+            for (int q = 0; q < (rank[s] + 15) / 16; ++q) {
+                net_f32x4 v = {};
+#pragma unroll 4
+                for (int c = wave; c < chunks; c += NW) {
+                    frag xf = {};
+                    if (slots[0] == s) xf = net_load_chunk(xp[0], c * KC + (lane >> 4) * E, d_in);
+                    v = net_mfma(as[(c * rank_frags + q) * 64], xf, v);
+                }
+                s_hp[wave][lane] = v;
+                __syncthreads();
+                if (wave == 0 && slots[0] == s && (lane & 15) < kProjOwnRows) {
+                    for (int i = 1; i < NW; ++i) v += s_hp[i][lane];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s_h[(lane & 15) * rp + q * 16 + (lane >> 4) * 4 + i] = v[i] * sc;
+                }
+                __syncthreads();
+            }
+        }
+    }
     __syncthreads();
     for (int q = wave; q < MF * NF; q += NW) {
         const int m = q / NF, f = q % NF;
@@ -528,12 +563,17 @@ void proj_few_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, in
             const B *bs = (const B *)(b + slot * b_slot) + (size_t)g * rp * 64 + (f0 + f) * 64 * E;
             const B *hr = (const B *)h + t * proj_geo<T>::parts * rp;
             for (int p = 0; p < chunks_r * 4; ++p) {        // E ranks at a time
-                const net_pack<B, E> hi = *(const net_pack<B, E> *)(hr + p * E);
-                net_pack<B, E> lo = {};
-                if constexpr (proj_geo<T>::parts == 2) lo = *(const net_pack<B, E> *)(hr + rp + p * E);
                 float hv[E];
+                if constexpr (OWN_H) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) hv[e] = net_f32(hi.v[e]) + (proj_geo<T>::parts == 2 ? net_f32(lo.v[e]) : 0.0f);
+                    for (int e = 0; e < E; ++e) hv[e] = s_h[(lane & 15) * rp + p * E + e];
+                } else {
+                    const net_pack<B, E> hi = *(const net_pack<B, E> *)(hr + p * E);
+                    net_pack<B, E> lo = {};
+                    if constexpr (proj_geo<T>::parts == 2) lo = *(const net_pack<B, E> *)(hr + rp + p * E);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) hv[e] = net_f32(hi.v[e]) + (proj_geo<T>::parts == 2 ? net_f32(lo.v[e]) : 0.0f);
+                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const B *bp = bs + ((p >> 2) * 256 + (p & 3) * 16 + (lane >> 4) * 4 + i) * E;
@@ -731,7 +771,9 @@ static void proj_launch(const psgpu_proj_t *p, const void *x, int64_t xs, const 
     const int32_t chunks = p->kp / proj_geo<T>::KC;
     int32_t *slots = nullptr;
     char *h = nullptr;
-    if (off) {
+    const int64_t t128 = (((int64_t)total + 127) / 128) * ((p->d_out + 127) / 128), t256 = (((int64_t)total + 255) / 256) * ((p->d_out + 127) / 128);
+    const bool own_h = off && total <= kProjOwnRows && t128 < 256;
+    if (off && !own_h) {
         slots = (int32_t *)work;
         h = work + proj_slot_bytes(total);
         proj_shrink<T>(p, x, xs, off, adapter, n_utt, total, slots, h, st);
@@ -740,7 +782,6 @@ static void proj_launch(const psgpu_proj_t *p, const void *x, int64_t xs, const 
     const size_t b_part = p->b_slot / proj_b_type<T>::parts;
     const uintptr_t at = (uintptr_t)x | (uintptr_t)(xs * sizeof(T));
     const bool near_rows = xs < ((int64_t)1 << 30) / 256 / (int64_t)sizeof(T);      // (a tile's rows at 32-bit offsets)
-    const int64_t t128 = (((int64_t)total + 127) / 128) * ((p->d_out + 127) / 128), t256 = (((int64_t)total + 255) / 256) * ((p->d_out + 127) / 128);
     const int dma = !near_rows ? 0 : (at & 15) == 0 ? 16 : (at & 3) == 0 ? 4 : 0;
 #define TILE(D, WM, WN, MF) do { \
         const int32_t tm = (int32_t)(((int64_t)total + WM * MF * 16 - 1) / (WM * MF * 16)), tn = (p->d_out + WN * 64 - 1) / (WN * 64); \
@@ -748,15 +789,19 @@ static void proj_launch(const psgpu_proj_t *p, const void *x, int64_t xs, const 
             b, p->b_slot, b_part, p->rp, p->rank, slots, h, (Y *)y, ys, tm, tn); \
     } while (0)
     if (t128 < 256) {
-        if (total <= 16) {
+#define FEW_REST p->a, p->a_slot, p->scale, p->max_adapters, off, adapter, n_utt
+        if (own_h) {
             const dim3 grid((uint32_t)((p->d_out + 63) / 64 * 4), 1);
-            proj_few_kernel<T, Y, 4, 1, 1><<<grid, 256, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, p->w, p->bias, p->d_out, b, p->b_slot, b_part, p->rp, p->rank, slots, h, (Y *)y, ys);
+            proj_few_kernel<T, Y, 4, 1, 1, true><<<grid, 256, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, p->w, p->bias, p->d_out, b, p->b_slot, b_part, p->rp, p->rank, slots, h, (Y *)y, ys, FEW_REST);
+        } else if (total <= 16) {
+            const dim3 grid((uint32_t)((p->d_out + 63) / 64 * 4), 1);
+            proj_few_kernel<T, Y, 4, 1, 1, false><<<grid, 256, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, p->w, p->bias, p->d_out, b, p->b_slot, b_part, p->rp, p->rank, slots, h, (Y *)y, ys, FEW_REST);
         } else if ((int64_t)((p->d_out + 63) / 64) * ((total + 31) / 32) < 512) {      // 512 rows to 1024: 19.5 against 20.8 us
             const dim3 grid((uint32_t)((p->d_out + 63) / 64), (uint32_t)((total + 15) / 16));
-            proj_few_kernel<T, Y, 4, 1, 4><<<grid, 256, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, p->w, p->bias, p->d_out, b, p->b_slot, b_part, p->rp, p->rank, slots, h, (Y *)y, ys);
+            proj_few_kernel<T, Y, 4, 1, 4, false><<<grid, 256, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, p->w, p->bias, p->d_out, b, p->b_slot, b_part, p->rp, p->rank, slots, h, (Y *)y, ys, FEW_REST);
         } else {
             const dim3 grid((uint32_t)((p->d_out + 63) / 64), (uint32_t)((total + 31) / 32));
-            proj_few_kernel<T, Y, 4, 2, 4><<<grid, 256, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, p->w, p->bias, p->d_out, b, p->b_slot, b_part, p->rp, p->rank, slots, h, (Y *)y, ys);
+            proj_few_kernel<T, Y, 4, 2, 4, false><<<grid, 256, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, p->w, p->bias, p->d_out, b, p->b_slot, b_part, p->rp, p->rank, slots, h, (Y *)y, ys, FEW_REST);
         }
     } else if (sizeof(T) == 4 || t256 < 1024) {
         if (dma == 16) TILE(16, 2, 2, 4); else if (dma == 4) TILE(4, 2, 2, 4); else TILE(0, 2, 2, 4);
@@ -764,6 +809,7 @@ static void proj_launch(const psgpu_proj_t *p, const void *x, int64_t xs, const 
         if constexpr (sizeof(T) == 2) { if (dma == 16) TILE(16, 2, 2, 8); else if (dma == 4) TILE(4, 2, 2, 8); else TILE(0, 2, 2, 8); }
     }
 #undef TILE
+#undef FEW_REST
 }
 
 extern "C" int psgpu_proj_run_dev(psgpu_proj_t *p, const void *x_dev, int64_t x_stride, const int32_t *utt_off_dev,

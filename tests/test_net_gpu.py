@@ -93,6 +93,47 @@ def test_projection_with_adapters(ci, dtype):
     _close(layer(x.cuda()), plain, perr, DT[dtype], "the shared projection alone")
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("lens, slots", [([4], [1]), ([1, 1, 1, 1], [2, 0, 2, 1]), ([1, 2], [-1, 3]), ([2, 0, 2], [0, 1, 2]), ([5], [2])])
+def test_projection_of_a_few_rows(lens, slots, dtype):
+    """up to four rows and more than that; several adapters, of the largest rank, one row of no utterance behind them"""
+    g = torch.Generator().manual_seed(440)
+    layer, w, b, ad = _layer(g, DT[dtype], 203, 330, [128, 7, 33], 128)
+    off = _off(lens)
+    for extra in (0, 1):
+        x = _rand(g, off[-1] + extra, 203, dtype=DT[dtype])
+        want, err = net_ref.proj(x, w, b, ad, off, slots)
+        out = torch.full((off[-1] + extra, 330), 5.0, dtype=DT[dtype], device="cuda")
+        layer(x.cuda(), _dev(off), _dev(slots), out=out)
+        _close(out[:off[-1]], want[:off[-1]], err[:off[-1]], DT[dtype], "y")
+        assert (out[off[-1]:] == 5.0).all()
+
+
+def test_rows_beyond_32_bit_offsets():
+    """the last rows of buffers of more than 2^31 elements: as those rows alone"""
+    g = torch.Generator(device="cuda").manual_seed(22)
+    n, w = 450000, 5120
+    x = torch.empty((n, w), dtype=torch.float16, device="cuda")
+    x[-3000:] = torch.randn(3000, w, generator=g, device="cuda").half()
+    x[:-3000] = 0.5
+    off = _dev([0, n - 3000, n - 1000, n])
+    assert n * w > 1 << 31
+    few = senone_scores(x[-3000:], want_best=True)
+    s, b = senone_scores(x, want_best=True)
+    assert torch.equal(s[-3000:], few[0]) and torch.equal(b[-3000:], few[1])
+    del s, b
+    few = group_norm(x[-3000:], _dev([0, 2000, 3000]), 32, act="silu").double()
+    y = group_norm(x, off, 32, act="silu")
+    # a step of float16, and twice what either may be off before its rounding: 1.2 * 5 u |z| + 8 u |z|, |z| below 8
+    assert ((y[-3000:].double() - few).abs() <= 2.0 ** -10 * few.abs() + 2 * 14 * net_ref.U * 8).all()
+    del y
+    layer = AdaptedProjection(torch.randn(64, w, generator=g, device="cuda").half() * w ** -0.5, None, 1, 8)
+    layer.set_adapter(0, torch.randn(8, w, generator=g, device="cuda").half() * w ** -0.5, torch.randn(64, 8, generator=g, device="cuda").half())
+    y = layer(x, off, _dev([-1, 0, -1]), out_dtype=torch.float32)
+    few = layer(x[-3000:], _dev([0, 2000, 3000]), _dev([0, -1]), out_dtype=torch.float32)
+    assert ((y[-3000:] - few).abs() <= 2 * 2 * net_ref.U * (w + 26) * 100).all()       # two orders of one sum, of magnitudes below 100
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("pad, shift", [(1, 0), (0, 1), (3, 5), (8, 8), (64, 0)])
 @pytest.mark.parametrize("rows", [3, 150])
