@@ -271,7 +271,7 @@ void gnorm_held_kernel(gn_args a)
 // results leave the next one's rows come into the registers that they free.  (Without that a compute unit's two workgroups load,
 // compute and store in step: 634 us for 384 k rows of 1024 in 32 groups.)  Neighbouring groups, which share lines of memory, run on
 // one die (workgroups are dealt to the 8 dies in turn; 577 -> 534 us).  384 k rows of 1024 in 32 groups with GELU: 505 us, 3.1 TB/s; some
-// 360 us of it are vector instructions, 30 a value.
+// 340 us of it are vector instructions, 28 a value.
 template <typename T, int NT, int NCH, int ACT>
 __global__ __launch_bounds__(NT, 4)
 void gnorm_stream_kernel(gn_args a)
@@ -363,7 +363,7 @@ void gnorm_stream_kernel(gn_args a)
     }
 }
 
-// ---- tiles of rows, in two passes: 102 k rows of 429 floats in 50 + 97 us, 3.5 TB/s ----------------------------------------------------------------------------------------------------
+// ---- tiles of rows, in two passes: 102 k rows of 429 floats in 47 + 95 us, 3.7 TB/s ----------------------------------------------------------------------------------------------------
 // Rows row .. tile_end - 1 begin in which utterance, and how far it reaches; false: no more utterances in the tile.  Partial sums lie
 // at tile + utterance: along the rows one of the two grows from piece to piece, so every piece has a place of its own.
 __device__ __forceinline__ bool gn_next(const gn_args &a, int &row, int tile_end, int &u, int &end)
@@ -458,7 +458,7 @@ void gnorm_apply_kernel(gn_args a)
 }
 
 // ---- which way ---------------------------------------------------------------------------------------------------------------------
-constexpr int kGnTiles = 2048;
+constexpr int kGnTiles = 4096;                          // (102 k rows of 429 floats: 142 us, with 2048 149)
 
 // rows of a tile: about kGnTiles tiles, of 16 rows or more
 static inline int32_t gn_tile_rows(int32_t total) { const int32_t r = (int32_t)(((int64_t)total + kGnTiles - 1) / kGnTiles); return r < 16 ? 16 : (r + 15) / 16 * 16; }

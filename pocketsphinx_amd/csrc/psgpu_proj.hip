@@ -218,13 +218,15 @@ void proj_shrink_few_kernel(const T *__restrict__ x, int64_t x_stride, int32_t t
         const uint64_t mine = __ballot(slot == s);
         todo &= ~mine;
         const frag *as = (const frag *)(a + s * a_slot) + lane;
+        const int used = (rank[s] + 15) / 16;           // (the ranks behind them are zeros)
         net_f32x4 acc[RF] = {};
 #pragma unroll 4
         for (int c = wave; c < chunks; c += 4) {
             frag f = {};
             if (mine >> col & 1) f = net_load_chunk(xr, c * KC + (lane >> 4) * E, d_in);
 #pragma unroll
-            for (int q = 0; q < RF; ++q) acc[q] = net_mfma(as[(c * rank_frags + min(q, rank_frags - 1)) * 64], f, acc[q]);
+            for (int q = 0; q < RF; ++q)
+                if (q < used) acc[q] = net_mfma(as[(c * rank_frags + q) * 64], f, acc[q]);
         }
 #pragma unroll
         for (int q = 0; q < RF; ++q) s_part[wave][q][lane] = acc[q];
