@@ -270,8 +270,8 @@ void gnorm_held_kernel(gn_args a)
 // As above, one group a slice, for slices that fill the registers: workgroups go from one (utterance, group) to the next, and while one's
 // results leave the next one's rows come into the registers that they free.  (Without that a compute unit's two workgroups load,
 // compute and store in step: 634 us for 384 k rows of 1024 in 32 groups.)  Neighbouring groups, which share lines of memory, run on
-// one die (workgroups are dealt to the 8 dies in turn; 577 -> 534 us).  384 k rows of 1024 in 32 groups with GELU: 505 us, 3.1 TB/s; some
-// 340 us of it are vector instructions, 28 a value.
+// one die (workgroups are dealt to the 8 dies in turn; 577 -> 534 us).  384 k rows of 1024 in 32 groups with GELU: 505 us, 3.1 TB/s; 280
+// us of it are vector instructions, 28 a value.
 template <typename T, int NT, int NCH, int ACT>
 __global__ __launch_bounds__(NT, 4)
 void gnorm_stream_kernel(gn_args a)

@@ -78,7 +78,7 @@ __device__ __forceinline__ unsigned long long scr_key(double v)
 __device__ __forceinline__ double scr_value(unsigned long long k) { return __longlong_as_double((long long)(k >> 63 ? k ^ 1ull << 63 : ~k)); }
 
 // A row a workgroup, NCH chunks of 16 bytes a work-item, in registers, the next row on its way; the priors are fetched once for all of
-// a workgroup's rows.  96 k rows of 5126 in bfloat16: 536 us, 3.7 TB/s; vector instructions, some 26 a value, are 370 us of it.
+// a workgroup's rows.  96 k rows of 5126 in bfloat16: 536 us, 3.7 TB/s; vector instructions, 29 a value, are 360 us of it.
 //
 // l in 32 bits, lf = fl(z - prior), keeps the order: the best l is among those whose lf is the greatest, and only those are taken in 64
 // bits.  A score's q = (top - l) unit + 1/2 in 32 bits is off by at most c + 6 q 2^-23, c = (2 |top| unit + 4) 2^-23: the three

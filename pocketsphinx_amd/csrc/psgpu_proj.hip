@@ -269,11 +269,11 @@ __device__ __forceinline__ void proj_expand(net_f32x4 (&acc)[4], bool mine, cons
 }
 
 // A tile of BM = WM MF 16 frames x BN = WN 64 outputs a workgroup; a wavefront MF 16 x 64.  A ring of three stages in LDS of 64 bytes
-// of the reduced axis: while one is multiplied the next is there or nearly and the one behind it is on its way (131072 rows of 1024 to
-// 1024 in bfloat16: 350 us, 786 TFLOP/s; LDS bounds it: 12 KB read and 3 KB written for 32 matrix instructions of a wavefront).  x lies in rows of 64
+// of the reduced axis: while one is multiplied the next is there or nearly and the one behind it is on its way.  x lies in rows of 64
 // bytes whose 16-byte pieces are exchanged by the row (piece p of row r at p ^ (r / 2 & 3)), so that 8 lanes meet no bank twice; W
-// lies as in memory.  Two workgroups a compute unit: one's first loads and last stores pass under the other's products (with one of
-// 256 x 256 they cost 18 us a tile, as much as 600 inputs' products).
+// lies as in memory.  131072 rows of 1024 to 1024 in bfloat16: with 256 x 256 a workgroup (8 wavefronts, one a compute unit) 335 us, 822
+// TFLOP/s; with 256 x 128 (two a compute unit, whose first loads and last stores pass under the other's products) 360 us: LDS
+// bounds both, for 32 matrix instructions of a wavefront 12 KB are read and 4 KB, there 6 KB, written.
 // DMA: x goes to LDS without a register, 16 bytes a lane where it is aligned to them, else 4 bytes (rows of 429 floats),
 // or 0: through registers.  A last stage that d_in does not fill goes through registers.
 // Where all of a tile's frames have one adapter its h and B are more stages of the same ring (h's parts against B's); else every
@@ -773,7 +773,7 @@ static void proj_launch(const psgpu_proj_t *p, const void *x, int64_t xs, const 
     const int32_t chunks = p->kp / proj_geo<T>::KC;
     int32_t *slots = nullptr;
     char *h = nullptr;
-    const int64_t t128 = (((int64_t)total + 127) / 128) * ((p->d_out + 127) / 128), t256 = (((int64_t)total + 255) / 256) * ((p->d_out + 127) / 128);
+    const int64_t t128 = (((int64_t)total + 127) / 128) * ((p->d_out + 127) / 128), t256 = (((int64_t)total + 255) / 256) * ((p->d_out + 255) / 256);
     const bool own_h = off && total <= kProjOwnRows && t128 < 256;
     if (off && !own_h) {
         slots = (int32_t *)work;
@@ -805,10 +805,10 @@ static void proj_launch(const psgpu_proj_t *p, const void *x, int64_t xs, const 
             const dim3 grid((uint32_t)((p->d_out + 63) / 64), (uint32_t)((total + 31) / 32));
             proj_few_kernel<T, Y, 4, 2, 4, false><<<grid, 256, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, p->w, p->bias, p->d_out, b, p->b_slot, b_part, p->rp, p->rank, slots, h, (Y *)y, ys, FEW_REST);
         }
-    } else if (sizeof(T) == 4 || t256 < 1024) {
+    } else if (sizeof(T) == 4 || t256 < 512 || round_up(p->d_out, 256) > p->d_out / 4 * 5) {       // (a quarter of the outputs' tiles in vain)
         if (dma == 16) TILE(16, 2, 2, 4); else if (dma == 4) TILE(4, 2, 2, 4); else TILE(0, 2, 2, 4);
     } else {
-        if constexpr (sizeof(T) == 2) { if (dma == 16) TILE(16, 2, 2, 8); else if (dma == 4) TILE(4, 2, 2, 8); else TILE(0, 2, 2, 8); }
+        if constexpr (sizeof(T) == 2) { if (dma == 16) TILE(16, 2, 4, 8); else if (dma == 4) TILE(4, 2, 4, 8); else TILE(0, 2, 4, 8); }
     }
 #undef TILE
 #undef FEW_REST
