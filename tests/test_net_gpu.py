@@ -109,6 +109,21 @@ def test_projection_of_a_few_rows(lens, slots, dtype):
         assert (out[off[-1]:] == 5.0).all()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d_out", [60, 100])
+def test_projection_of_many_rows_to_few_outputs(d_out, dtype):
+    g = torch.Generator().manual_seed(450)
+    layer, w, b, ad = _layer(g, DT[dtype], 77, d_out, [20, 0, 5], 20)
+    lens, slots = [9000, 1, 0, 1, 40, 8000], [0, 2, 0, 0, -1, 2]
+    off = _off(lens, start=2)
+    x = _rand(g, off[-1] + 3, 77, dtype=DT[dtype])
+    want, err = net_ref.proj(x, w, b, ad, off, slots)
+    out = torch.full((off[-1] + 3, d_out), 5.0, dtype=DT[dtype], device="cuda")
+    layer(x.cuda(), _dev(off), _dev(slots), out=out)
+    _close(out[2:off[-1]], want[2:off[-1]], err[2:off[-1]], DT[dtype], "y")
+    assert (out[:2] == 5.0).all() and (out[off[-1]:] == 5.0).all()
+
+
 def test_rows_beyond_32_bit_offsets():
     """the last rows of buffers of more than 2^31 elements: as those rows alone"""
     g = torch.Generator(device="cuda").manual_seed(22)
@@ -377,6 +392,7 @@ GN = [
     ([2, 0, 5, 1, 9] * 60, 301, 43, "silu", 1e-5),
     ([1] * 512, 17000, 1, "none", 1e-5),
     ([3000, 0, 1, 2, 70, 13000], 512, 128, "silu", 1e-5),
+    ([3000, 0, 5000, 1, 14000, 700], 1024, 128, "gelu", 1e-5),
 ]
 
 
@@ -526,6 +542,28 @@ def test_senone_scores(rows, n_sen, dtype):
         assert s.dtype == torch.int16 and np.array_equal(s.cpu().numpy(), ws)
         assert (np.abs(b.double().cpu().numpy() - wb) <= be).all()
         assert torch.equal(senone_scores(z.cuda(), None if p is None else p.cuda(), scale=scale, logbase=base), s)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows, n_sen", [(600, 100), (1500, 2050), (530, 5126), (520, 3500), (515, 8190), (3, 45000), (600, 5)])
+def test_senone_scores_of_many_rows_and_long_ones(rows, n_sen, dtype):
+    """with masked senones, NaN, infinities and rows of nothing in between"""
+    g = torch.Generator().manual_seed(500 + n_sen)
+    z = _rand(g, rows, n_sen, dtype=DT[dtype], scale=4.0)
+    inf, k = float("inf"), rows // 3
+    z[0, 1:] = -inf
+    z[1] = -inf
+    z[2] = torch.finfo(DT[dtype]).min
+    if k > 2:
+        z[k] = float("nan"); z[k + 1, ::3] = -inf; z[k + 2, n_sen - 1] = float("nan"); z[k + 3, n_sen // 2] = inf; z[k + 4, 0] = torch.finfo(DT[dtype]).max
+    prior = torch.log_softmax(_rand(g, n_sen).double(), 0).float()
+    ws, wb, be = net_ref.senones(z, prior, 0.8, 1.0001)
+    s, b = senone_scores(z.cuda(), prior.cuda(), scale=0.8, want_best=True)
+    assert np.array_equal(s.cpu().numpy(), ws)
+    b = b.double().cpu().numpy()
+    fin = np.isfinite(wb)
+    assert (np.abs(b[fin] - wb[fin]) <= be[fin] + np.abs(wb[fin]) * 2.0 ** -22).all()
+    assert b[1] == -inf and (k <= 2 or (np.isnan(b[k]) and np.isnan(b[k + 2])))
 
 
 @pytest.mark.parametrize("pad, shift", [(1, 0), (0, 1), (3, 5), (8, 0)])
