@@ -1225,7 +1225,7 @@ int psgpu_group_norm_dev(int32_t dtype, const void *x_dev, int64_t x_stride, con
  * the scaled log-likelihood over the frame's best in the units of the reference's scores (-logbase, SENSCR_SHIFT), lower is better;
  * taken in 64 bits.  The rows are normalised over all senones (as with -compallsen) and serve as un-normalised rows alike.  -inf, a
  * masked senone: 32767; a NaN counts as -inf here.  best_dev [total_frames] float or NULL: max l[t] - log sum exp z[t], the best
- * senone's log-likelihood (-inf where every senone is masked, NaN where an output is). */
+ * senone's log-likelihood (-inf where every senone is masked, NaN where an output is NaN or +inf), to 2^-52 of the greatest z at best. */
 int psgpu_senone_scores_dev(int32_t dtype, const void *logits_dev, int64_t logits_stride, int32_t total_frames, int32_t n_sen,
                             const float *log_prior_dev, double scale, double logbase, int16_t *senscr_dev, int64_t senscr_stride,
                             float *best_dev, void *stream);

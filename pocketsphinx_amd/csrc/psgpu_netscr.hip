@@ -89,7 +89,9 @@ __device__ __forceinline__ double scr_value(unsigned long long k) { return __lon
 // not finite, all scores are taken in 64 bits.
 //
 // The softmax's sum: exp(z - m) = 2^(z a - m a) in one fused step, a = log2(e) in 32 bits; m a rounded is b, which all terms share, and
-// the logarithm gets b - m a back in 64 bits.
+// the logarithm gets b - m a back in 64 bits.  b - m a is up to half of b's last place, and 2 to it a factor of all terms: for m up to 1e6 one
+// of 2^(1/16), beyond 1e10 one that leaves float's range.  A row whose m is beyond 1e6 (masked as a whole by a low finite value, say)
+// takes 2^((z - m) a) instead, from memory.
 template <typename T, int NT, int NCH>
 __global__ __launch_bounds__(NT, 4)
 void netscr_row_kernel(const T *__restrict__ z, int64_t z_stride, int32_t rows, int32_t n_sen, const float *__restrict__ prior, double unit,
@@ -168,7 +170,7 @@ void netscr_row_kernel(const T *__restrict__ z, int64_t z_stride, int32_t rows, 
             atomicMax(&s_top[par], scr_key(mine));
         }
         const float a = 1.4426950408889634f;
-        const bool huge = !(fabsf(mz) < 1e38f);             // m a could leave float's range; values that far apart are equal or e^-(1e30)
+        const bool huge = !(fabsf(mz) < 1e6f);
         const float b = huge ? 0.0f : mz * a;
         double total = 0.0;
         if (best) {
@@ -186,7 +188,7 @@ void netscr_row_kernel(const T *__restrict__ z, int64_t z_stride, int32_t rows, 
 #pragma unroll 1
                 for (int s = tid; s < n_sen; s += NT) {
                     const float ze = net_f32(row[s]);
-                    sum += ze == mz ? 1.0f : ze != ze ? ze : 0.0f;
+                    sum += ze == mz ? 1.0f : __builtin_amdgcn_exp2f((ze - mz) * a);       // (also for two infinities)
                 }
             }
             total = sum;
