@@ -242,7 +242,8 @@ void proj_shrink_few_kernel(const T *__restrict__ x, int64_t x_stride, int32_t t
 }
 
 // ---- the product in tiles -----------------------------------------------------------------------------------------------------------
-// acc of 16 frames (column lane & 15) += B_s h over the ranks of adapter s, for the frames whose slot it is
+// acc of 16 frames (column lane & 15) += B_s h over the ranks of adapter s, for the frames whose slot it is; the others' h is zero here,
+// and what they held is put back behind the products: an infinity in B_s makes a NaN of zero
 template <typename T>
 __device__ __forceinline__ void proj_expand(net_f32x4 (&acc)[4], bool mine, const char *bs, size_t b_part, int chunks, const char *ht, int rp)
 {
@@ -250,6 +251,9 @@ __device__ __forceinline__ void proj_expand(net_f32x4 (&acc)[4], bool mine, cons
     typedef typename proj_b_type<T>::type B;
     typedef typename net_frag<B>::type bfrag;
     const int lane = threadIdx.x & 63;
+    net_f32x4 was[4];
+#pragma unroll
+    for (int f = 0; f < 4; ++f) was[f] = acc[f];
 #pragma unroll 1
     for (int c = 0; c < chunks; ++c) {
         bfrag hi = {}, lo = {};
@@ -266,6 +270,9 @@ __device__ __forceinline__ void proj_expand(net_f32x4 (&acc)[4], bool mine, cons
             if constexpr (proj_b_type<T>::parts == 2) acc[f] = net_mfma(((const bfrag *)(bs + b_part))[(c * 4 + f) * 64 + lane], hi, acc[f]);
         }
     }
+    if (!mine)
+#pragma unroll
+        for (int f = 0; f < 4; ++f) acc[f] = was[f];
 }
 
 // A tile of BM = WM MF 16 frames x BN = WN 64 outputs a workgroup; a wavefront MF 16 x 64.  A ring of three stages in LDS of 64 bytes

@@ -6,7 +6,7 @@ import torch
 
 import net_ref
 from pocketsphinx_amd import senone_scores
-from test_net_gpu import DT, _rand
+from test_net_gpu import DT, _close, _dev, _layer, _off, _rand
 
 pytestmark = pytest.mark.gpu
 
@@ -65,3 +65,40 @@ def test_best_of_every_non_finite_row(n_sen, dtype):
     assert np.array_equal(s.cpu().numpy(), ws)
     for r in (1, 4, 8):
         assert abs(float(b[r]) - wb[r]) <= be[r]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows", [3, 100, 1000, 6500])
+def test_a_non_finite_adapter_stays_with_its_utterances(rows, dtype):
+    """few rows, tiles of 128 and of 256 frames: infinities and NaN in one speaker's a or b show in that speaker's frames, in the outputs they
+    feed, and nowhere else; the batch interleaves the speakers, so tiles hold several"""
+    g = torch.Generator().manual_seed(620)
+    d_in, d_out = 136, 5126
+    layer, w, b, ad = _layer(g, DT[dtype], d_in, d_out, [16, 3, 20, 16], 40)
+    lens = [1, rows // 5, 0, 1, rows // 3, 1]
+    lens += [1] * min(rows, 40)
+    lens += [max(0, rows - sum(lens))]
+    slots = [(2 * u + 1) % 5 - 1 for u in range(len(lens))]             # -1 .. 3
+    off = _off(lens)
+    x = _rand(g, off[-1], d_in, dtype=DT[dtype])
+    want, err = net_ref.proj(x, w, b, ad, off, slots)
+    row_slot = torch.tensor([slots[u] for u, n in enumerate(lens) for _ in range(n)])
+    inf, nan = float("inf"), float("nan")
+    a1, b1, s1 = ad[1]
+    b1 = b1.clone()
+    b1[7, 1], b1[2500, 2], b1[d_out - 1, 0] = inf, nan, -inf
+    layer.set_adapter(1, a1, b1, s1)
+    a2, b2, s2 = ad[2]
+    a2 = a2.clone()
+    a2[19, d_in - 1], a2[0, 3] = inf, nan
+    layer.set_adapter(2, a2, b2, s2)
+    for out_dtype in {DT[dtype], torch.float32}:
+        got = layer(x.cuda(), _dev(off), _dev(slots), out_dtype=out_dtype).double().cpu()
+        other = (row_slot != 1) & (row_slot != 2)
+        _close(got[other], want[other], err[other], out_dtype, "other speakers")
+        hit = torch.zeros(d_out, dtype=torch.bool)
+        hit[[7, 2500, d_out - 1]] = True
+        one = got[row_slot == 1]
+        assert not torch.isfinite(one[:, hit]).any()
+        _close(one[:, ~hit], want[row_slot == 1][:, ~hit], err[row_slot == 1][:, ~hit], out_dtype, "the outputs that the infinity does not feed")
+        assert not torch.isfinite(got[row_slot == 2]).any()
