@@ -14,9 +14,12 @@
 // zeros in the padding.  The outputs are dealt to the rows of four fragments so that one store of a wavefront writes 64 neighbouring
 // bytes of each of 16 frames (proj_out_of).
 //
-// The adapters' h is kept in 32 bits, for the half types as two bfloat16 parts (their sum is h to 2^-17) that go through the matrix
-// instructions as one more piece of the reduced axis, against B in bfloat16: float16's B is two parts (exact), of whose products the
-// smallest, 2^-16 of the term, is left out.  In float16 itself h could overflow.
+// The adapters' h is kept in 32 bits, for the half types as three bfloat16 parts of 8 bits each, cut, not rounded, so that their sum is h
+// exactly.  They go through the matrix instructions as more pieces of the reduced axis, against B in bfloat16: float16's B is two
+// parts (exact); the product of the smallest two, 2^-25 of the term, is left out.  In float16 itself h could overflow.  (Two parts
+// were 2^-18 of h, an adapter's term in 32 bits off by 1.3e-6 of its size, 10 times what its sums are.  The third costs 22 of 1058 us for
+// 384 k rows of 1024 to 1024 in bfloat16 with rank 32, the two more 18 of 660 us for 48 k rows of 1024 to 5126 in float16.)
+// A value that is not finite is a third part alone: against B's second part, often 0, an infinity would be a NaN.
 #include "psgpu_net_dev.h"
 #include <cmath>
 #include <cstring>
@@ -41,7 +44,8 @@ constexpr int kProjNoRow = -2;                      // rows of no utterance: lef
 template <typename T> struct proj_geo {
     static constexpr int E = 16 / sizeof(T);        // elements a lane, elements a chunk
     static constexpr int KC = 4 * E;
-    static constexpr int parts = sizeof(T) == 4 ? 1 : 2;    // of h
+    static constexpr int parts = sizeof(T) == 4 ? 1 : 3;    // of h
+    static constexpr int h_bytes = sizeof(T) == 4 ? 4 : 6;  // an h takes in all its parts
     typedef typename net_frag<T>::type frag;
 };
 template <typename T> struct proj_b_type { typedef psg_bf16 type; static constexpr int parts = 1; };     // what B is kept in
@@ -55,12 +59,22 @@ __device__ __forceinline__ int proj_out_of(int f, int m)
     return sizeof(T) == 4 ? f * 16 + m : (f >> 1) * 32 + (m >> 2) * 8 + (f & 1) * 4 + (m & 3);
 }
 
-// the two bfloat16 parts of a value (an infinity has a second part of 0)
+// the two bfloat16 parts of a float16 (an infinity has a second part of 0)
 __device__ __forceinline__ void proj_split(float v, psg_bf16 &hi, psg_bf16 &lo)
 {
     hi = net_cast<psg_bf16>(v);
     const float rest = v - net_f32(hi);
     lo = net_cast<psg_bf16>(__builtin_isinf(net_f32(hi)) ? 0.0f : rest);
+}
+
+// the three bfloat16 parts of a float
+__device__ __forceinline__ void proj_split3(float v, psg_bf16 &hi, psg_bf16 &mid, psg_bf16 &lo)
+{
+    const bool fin = __builtin_isfinite(v);
+    const float a = fin ? __uint_as_float(__float_as_uint(v) & 0xffff0000u) : 0.0f, b = __uint_as_float(__float_as_uint(fin ? v - a : 0.0f) & 0xffff0000u);
+    hi.bits = (uint16_t)(__float_as_uint(a) >> 16);
+    mid.bits = (uint16_t)(__float_as_uint(b) >> 16);
+    lo = net_cast<psg_bf16>((v - a) - b);
 }
 
 // ---- layouts, one 16-byte lane's share a work-item --------------------------------------------------------------------------------
@@ -133,11 +147,13 @@ __device__ __forceinline__ void proj_store_h(net_f32x4 v, float scale, char *h, 
         for (int i = 0; i < 4; ++i) o[i] = v[i] * scale;
         *(net_f32x4 *)((float *)h + t * rp + r) = o;
     } else {
-        net_pack<psg_bf16, 4> hi, lo;
+        net_pack<psg_bf16, 4> hi, mid, lo;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) proj_split(v[i] * scale, hi.v[i], lo.v[i]);
-        *(uint64_t *)((psg_bf16 *)h + t * 2 * rp + r) = __builtin_bit_cast(uint64_t, hi);
-        *(uint64_t *)((psg_bf16 *)h + t * 2 * rp + rp + r) = __builtin_bit_cast(uint64_t, lo);
+        for (int i = 0; i < 4; ++i) proj_split3(v[i] * scale, hi.v[i], mid.v[i], lo.v[i]);
+        psg_bf16 *to = (psg_bf16 *)h + t * 3 * rp + r;
+        *(uint64_t *)to = __builtin_bit_cast(uint64_t, hi);
+        *(uint64_t *)(to + rp) = __builtin_bit_cast(uint64_t, mid);
+        *(uint64_t *)(to + 2 * rp) = __builtin_bit_cast(uint64_t, lo);
     }
 }
 
@@ -256,18 +272,20 @@ __device__ __forceinline__ void proj_expand(net_f32x4 (&acc)[4], bool mine, cons
     for (int f = 0; f < 4; ++f) was[f] = acc[f];
 #pragma unroll 1
     for (int c = 0; c < chunks; ++c) {
-        bfrag hi = {}, lo = {};
-        if (mine) {
-            const B *hr = (const B *)ht + c * KC + (lane >> 4) * E;
-            hi = *(const bfrag *)hr;
-            if constexpr (proj_geo<T>::parts == 2) lo = *(const bfrag *)(hr + rp);
-        }
+        bfrag hp[proj_geo<T>::parts] = {};
+        if (mine)
+#pragma unroll
+            for (int i = 0; i < proj_geo<T>::parts; ++i) hp[i] = *(const bfrag *)((const B *)ht + i * rp + c * KC + (lane >> 4) * E);
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
             const bfrag w = ((const bfrag *)bs)[(c * 4 + f) * 64 + lane];
-            acc[f] = net_mfma(w, hi, acc[f]);
-            if constexpr (proj_geo<T>::parts == 2) acc[f] = net_mfma(w, lo, acc[f]);
-            if constexpr (proj_b_type<T>::parts == 2) acc[f] = net_mfma(((const bfrag *)(bs + b_part))[(c * 4 + f) * 64 + lane], hi, acc[f]);
+#pragma unroll
+            for (int i = 0; i < proj_geo<T>::parts; ++i) acc[f] = net_mfma(w, hp[i], acc[f]);
+            if constexpr (proj_b_type<T>::parts == 2) {
+                const bfrag w2 = ((const bfrag *)(bs + b_part))[(c * 4 + f) * 64 + lane];
+                acc[f] = net_mfma(w2, hp[0], acc[f]);
+                acc[f] = net_mfma(w2, hp[1], acc[f]);
+            }
         }
     }
     if (!mine)
@@ -347,22 +365,22 @@ void proj_tile_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, i
             return;
         }
         const uint32_t to = lds + buf * ST;
-        // the last stage of d_in, or an adapter's: B's parts 0, 0, 1 against h's 0, 1, 0
+        // the last stage of d_in, or an adapter's: B's parts 0, 0, 0, 1, 1 against h's 0, 1, 2, 0, 1
         const bool own = st < stages;
         const int part = own ? 0 : (st - stages) / rchunks, c = own ? st : (st - stages) - part * rchunks;
         const size_t group = own ? (size_t)chunks * 4096 : (size_t)rp * 64 * sizeof(typename proj_b_type<T>::type);
-        const char *ws = (own ? wt : b + slot0 * b_slot + (part == 2 ? b_part : 0) + (size_t)g0 * group) + (size_t)c * 4096;
+        const char *ws = (own ? wt : b + slot0 * b_slot + (part >= 3 ? b_part : 0) + (size_t)g0 * group) + (size_t)c * 4096;
 #pragma unroll
         for (int i = 0; i < WI; ++i) {
             const int q = wave * WI + i;
             net_load_lds<16>(ws + (size_t)(q >> 2) * group + (q & 3) * 1024, lane * 16, to + XB + q * 1024);
         }
-        const char *hs = h + (size_t)m0 * rp * 4 + (part == 1 ? rp * 2 : 0) + (size_t)c * 64;
+        const char *hs = h + (size_t)m0 * rp * proj_geo<T>::h_bytes + (part >= 3 ? part - 3 : part) * rp * 2 + (size_t)c * 64;
 #pragma unroll 1
         for (int i = 0; i < XI; ++i) {
             const int64_t r = min((int64_t)(wave * XI + i) * 16 + (lane >> 2), (int64_t)rows - 1 - m0);
             if (own) *(frag *)(s_buf + buf * ST + (wave * XI + i) * 1024 + lane * 16) = net_load_chunk(x + (m0 + r) * x_stride, st * KC + xk, d_in);
-            else net_load_lds<16>(hs, (uint32_t)((int)r * rp * 4 + xk * (int)sizeof(T)), to + (wave * XI + i) * 1024);
+            else net_load_lds<16>(hs, (uint32_t)((int)r * rp * proj_geo<T>::h_bytes + xk * (int)sizeof(T)), to + (wave * XI + i) * 1024);
         }
     };
     auto put = [&](int st, int buf) {                       // the pieces that came through registers
@@ -388,7 +406,7 @@ void proj_tile_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, i
         mixed = !__syncthreads_and(same);
         if (!mixed && slot0 >= 0) {
             rchunks = (rank[slot0] + KC - 1) / KC;
-            total += rchunks * (sizeof(T) == 4 ? 1 : 1 + proj_b_type<T>::parts);
+            total += rchunks * (proj_geo<T>::parts + (proj_b_type<T>::parts == 2 ? 2 : 0));
         }
         if (stages == 1 && total > 1) fetch(1, 1);
     }
@@ -443,7 +461,7 @@ void proj_tile_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, i
             while (todo) {
                 const int s = __shfl(slot[m], __builtin_ctzll(todo));
                 todo &= ~__ballot(slot[m] == s);
-                proj_expand<T>(acc[m], slot[m] == s, bg + s * b_slot, b_part, (rank[s] + KC - 1) / KC, h + (size_t)t[m] * rp * 4, rp);
+                proj_expand<T>(acc[m], slot[m] == s, bg + s * b_slot, b_part, (rank[s] + KC - 1) / KC, h + (size_t)t[m] * rp * proj_geo<T>::h_bytes, rp);
             }
         }
     }
@@ -577,11 +595,14 @@ void proj_few_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, in
 #pragma unroll
                     for (int e = 0; e < E; ++e) hv[e] = s_h[(lane & 15) * rp + p * E + e];
                 } else {
-                    const net_pack<B, E> hi = *(const net_pack<B, E> *)(hr + p * E);
-                    net_pack<B, E> lo = {};
-                    if constexpr (proj_geo<T>::parts == 2) lo = *(const net_pack<B, E> *)(hr + rp + p * E);
+                    net_pack<B, E> hp[proj_geo<T>::parts];
 #pragma unroll
-                    for (int e = 0; e < E; ++e) hv[e] = net_f32(hi.v[e]) + (proj_geo<T>::parts == 2 ? net_f32(lo.v[e]) : 0.0f);
+                    for (int i = 0; i < proj_geo<T>::parts; ++i) hp[i] = *(const net_pack<B, E> *)(hr + i * rp + p * E);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        hv[e] = net_f32(hp[0].v[e]);
+                        if constexpr (proj_geo<T>::parts == 3) hv[e] = (hv[e] + net_f32(hp[1].v[e])) + net_f32(hp[2].v[e]);      // exact
+                    }
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -741,13 +762,13 @@ extern "C" int psgpu_proj_set_adapter(psgpu_proj_t *p, int32_t slot, int32_t ran
 extern "C" int32_t psgpu_proj_d_in(const psgpu_proj_t *p) { return p ? p->d_in : PSGPU_EINVAL; }
 extern "C" int32_t psgpu_proj_d_out(const psgpu_proj_t *p) { return p ? p->d_out : PSGPU_EINVAL; }
 
-// workspace: row_slot [total], then h [total][rp]
+// workspace: row_slot [total], then h [total][parts][rp]
 static inline size_t proj_slot_bytes(int32_t total) { return ((size_t)total * 4 + 255) / 256 * 256; }
 
 extern "C" size_t psgpu_proj_work_bytes(const psgpu_proj_t *p, int32_t total_frames)
 {
     if (!p || total_frames <= 0) return 0;
-    return proj_slot_bytes(total_frames) + (size_t)total_frames * p->rp * 4;
+    return proj_slot_bytes(total_frames) + (size_t)total_frames * p->rp * (p->dtype == PSGPU_DT_F32 ? proj_geo<float>::h_bytes : proj_geo<psg_half>::h_bytes);
 }
 
 template <typename T>

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import net_ref
-from pocketsphinx_amd import senone_scores
+from pocketsphinx_amd import AdaptedProjection, senone_scores
 from test_net_gpu import DT, _close, _dev, _layer, _off, _rand
 
 pytestmark = pytest.mark.gpu
@@ -102,3 +102,70 @@ def test_a_non_finite_adapter_stays_with_its_utterances(rows, dtype):
         assert not torch.isfinite(one[:, hit]).any()
         _close(one[:, ~hit], want[row_slot == 1][:, ~hit], err[row_slot == 1][:, ~hit], out_dtype, "the outputs that the infinity does not feed")
         assert not torch.isfinite(got[row_slot == 2]).any()
+
+
+def _as_32_bits(got, want, terms, what):
+    """the root mean square of the error against that of the values.  A sum of n products of like size kept in 32 bits: after i of them the
+    sum is about sqrt(i) of one, and adding the next rounds it by at most U, U / sqrt 3 in the mean square; the n errors add up to
+    U n / sqrt 6 of one product, U sqrt(n / 6) of the sum.  `terms`: of the sums that feed one another, one after another; the store to 32 bits
+    is U / sqrt 3."""
+    rel = float(((got.double() - want) ** 2).mean().sqrt() / (want ** 2).mean().sqrt())
+    assert rel <= net_ref.U * (sum(terms) / 6 + 1 / 3) ** 0.5, "%s: off by %.3g, %.3g is 32 bits' due" % (what, rel, net_ref.U * (sum(terms) / 6 + 1 / 3) ** 0.5)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows, d_in, d_out", [(3, 1024, 1024), (40, 1024, 1024), (1000, 256, 5126), (6500, 256, 5126), (6500, 1024, 5126)])
+def test_sums_keep_32_bits(rows, d_in, d_out, dtype):
+    """into float32: the shared product, the adapter's alone, of one adapter for all frames and of several in a tile"""
+    g = torch.Generator().manual_seed(630)
+    w = _rand(g, d_out, d_in, dtype=DT[dtype], scale=d_in ** -0.5)
+    ad = [(_rand(g, 32, d_in, dtype=DT[dtype], scale=d_in ** -0.5), _rand(g, d_out, 32, dtype=DT[dtype])) for _ in range(2)]
+    x = _rand(g, rows, d_in, dtype=DT[dtype]).cuda()
+    xd = x.double()
+    _as_32_bits(AdaptedProjection(w)(x, out_dtype=torch.float32), xd @ w.cuda().double().t(), [d_in], "the shared product")
+    alone = AdaptedProjection(torch.zeros_like(w), None, 2, 32)
+    term = []
+    for k, (a, b) in enumerate(ad):
+        alone.set_adapter(k, a, b)
+        term.append((xd @ a.cuda().double().t()) @ b.cuda().double().t())
+    _as_32_bits(alone(x, _dev([0, rows]), _dev([1]), out_dtype=torch.float32), term[1], [d_in, 5 * 32], "one adapter")
+    slots = torch.arange(rows) % 2
+    want = torch.where(slots.cuda()[:, None] == 0, term[0], term[1])
+    _as_32_bits(alone(x, _dev(list(range(rows + 1))), _dev(slots.tolist()), out_dtype=torch.float32), want, [d_in, 5 * 32], "two adapters")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_a_frames_answer_hardly_hangs_on_its_batch(dtype):
+    """the same frames among two, few, many of their own speaker and many of others: sums in another order, each in 32 bits"""
+    g = torch.Generator().manual_seed(640)
+    d_in, d_out = 512, 5126
+    layer = AdaptedProjection(torch.zeros(d_out, d_in, dtype=DT[dtype]), None, 2, 24)
+    for k in range(2):
+        layer.set_adapter(k, _rand(g, 24, d_in, dtype=DT[dtype], scale=d_in ** -0.5), _rand(g, d_out, 24, dtype=DT[dtype]))
+    x = _rand(g, 6500, d_in, dtype=DT[dtype]).cuda()
+    first = layer(x[:2], _dev([0, 2]), _dev([1]), out_dtype=torch.float32).double()
+    for n in (40, 1000, 6500):
+        _as_32_bits(layer(x[:n], _dev([0, n]), _dev([1]), out_dtype=torch.float32)[:2], first, [2 * d_in, 2 * 5 * 24], "%d frames" % n)
+        _as_32_bits(layer(x[:n], _dev([0, 2, n]), _dev([1, 0]), out_dtype=torch.float32)[:2], first, [2 * d_in, 2 * 5 * 24], "%d frames of two" % n)
+
+
+@pytest.mark.parametrize("rows", [2, 40, 1000, 6500])
+def test_an_infinite_input_of_float16(rows):
+    """an infinity in x goes through a (of one rank) and b as the formula says; b's values have a second part of 0 here"""
+    g = torch.Generator().manual_seed(650)
+    d_in, d_out, r = 136, 5126, 32
+    layer = AdaptedProjection(torch.zeros(d_out, d_in, dtype=torch.float16), None, 1, r)
+    a, b = _rand(g, r, d_in, dtype=torch.float16).abs() + 1, torch.sign(_rand(g, d_out, 1, dtype=torch.float16)).expand(d_out, r).contiguous()
+    layer.set_adapter(0, a, b)
+    x = torch.zeros(rows, d_in, dtype=torch.float16)
+    x[:, 2] = 1.0
+    x[rows - 1, 2] = float("inf")
+    y = layer(x.cuda(), _dev([0, rows]), _dev([0])).cpu()
+    # (W is 0 and meets the infinity: the shared product alone makes NaN of that row)
+    assert torch.isnan(y[rows - 1]).all() and torch.isfinite(y[:rows - 1]).all()
+    layer = AdaptedProjection(torch.ones(d_out, 1, dtype=torch.float16).mul_(b[:, :1]).expand(d_out, d_in).contiguous(), None, 1, r)
+    layer.set_adapter(0, a, b)
+    x[rows - 1] = 1.0
+    x[rows - 1, 2] = float("inf")
+    y = layer(x.cuda(), _dev([0, rows]), _dev([0])).cpu()
+    assert torch.equal(y[rows - 1].float(), b[:, 0].float() * float("inf"))
