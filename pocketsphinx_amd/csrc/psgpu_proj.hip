@@ -138,9 +138,13 @@ __device__ __forceinline__ int proj_slot_of_rows(const int32_t *utt_off, const i
 }
 
 // ---- h --------------------------------------------------------------------------------------------------------------------------------
+// ranks r .. r + 3 of frame t.  Those from `rank` on are 0, whatever A's padding made of an infinity: B's padding would make a NaN of it
 template <typename T>
-__device__ __forceinline__ void proj_store_h(net_f32x4 v, float scale, char *h, size_t t, int rp, int r)
+__device__ __forceinline__ void proj_store_h(net_f32x4 v, float scale, char *h, size_t t, int rp, int r, int rank)
 {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (r + i >= rank) v[i] = 0.0f;
     if constexpr (sizeof(T) == 4) {
         net_f32x4 o;
 #pragma unroll
@@ -200,12 +204,13 @@ void proj_shrink_kernel(const T *__restrict__ x, int64_t x_stride, int32_t total
             }
         }
         const float sc = scale[s];
+        const int rank_of = rank[s];
 #pragma unroll
         for (int m = 0; m < MR; ++m)
             if (mine >> (m * 16 + (lane & 15)) & 1)
 #pragma unroll
                 for (int q = 0; q < RF; ++q)
-                    if (q < rank_frags) proj_store_h<T>(acc[m][q], sc, h, (size_t)row0 + m * 16 + (lane & 15), rp, q * 16 + (lane >> 4) * 4);
+                    if (q < rank_frags) proj_store_h<T>(acc[m][q], sc, h, (size_t)row0 + m * 16 + (lane & 15), rp, q * 16 + (lane >> 4) * 4, rank_of);
     }
 }
 
@@ -251,7 +256,7 @@ void proj_shrink_few_kernel(const T *__restrict__ x, int64_t x_stride, int32_t t
         for (int q = wave; q < rank_frags; q += 4) {
             net_f32x4 v = s_part[0][q][lane];
             for (int w = 1; w < 4; ++w) v += s_part[w][q][lane];
-            if (mine >> col & 1) proj_store_h<T>(v, sc, h, (size_t)row0 + col, rp, q * 16 + (lane >> 4) * 4);
+            if (mine >> col & 1) proj_store_h<T>(v, sc, h, (size_t)row0 + col, rp, q * 16 + (lane >> 4) * 4, rank[s]);
         }
         __syncthreads();
     }
@@ -568,7 +573,10 @@ void proj_few_kernel(const T *__restrict__ x, int64_t x_stride, int32_t rows, in
                 if (wave == 0 && slots[0] == s && (lane & 15) < kProjOwnRows) {
                     for (int i = 1; i < NW; ++i) v += s_hp[i][lane];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s_h[(lane & 15) * rp + q * 16 + (lane >> 4) * 4 + i] = v[i] * sc;
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = q * 16 + (lane >> 4) * 4 + i;
+                        s_h[(lane & 15) * rp + r] = r < rank[s] ? v[i] * sc : 0.0f;       // (as proj_store_h)
+                    }
                 }
                 __syncthreads();
             }

@@ -169,3 +169,29 @@ def test_an_infinite_input_of_float16(rows):
     x[rows - 1, 2] = float("inf")
     y = layer(x.cuda(), _dev([0, rows]), _dev([0])).cpu()
     assert torch.equal(y[rows - 1].float(), b[:, 0].float() * float("inf"))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rank", [1, 5, 33])
+@pytest.mark.parametrize("rows, d_out", [(3, 330), (40, 330), (1000, 5126), (6500, 5126), (20000, 60)])
+def test_non_finite_inputs_go_through_as_the_formula_says(rows, d_out, rank, dtype):
+    """rows of one speaker and of two in turn with an infinity or a NaN in x: every output as in 64 bits, non-finite ones alike"""
+    g = torch.Generator().manual_seed(660 + rank)
+    d_in = 75
+    w = _rand(g, d_out, d_in, dtype=DT[dtype])
+    layer = AdaptedProjection(w, None, 2, 40)
+    ad = {}
+    for k in range(2):          # one sign in a row of b and in a: an infinity's terms do not meet one of the other sign among the ranks
+        ad[k] = (_rand(g, rank, d_in, dtype=DT[dtype]).abs() + 0.5, (torch.sign(_rand(g, d_out, 1)) * (_rand(g, d_out, rank).abs() + 0.5)).to(DT[dtype]), 0.5)
+        layer.set_adapter(k, *ad[k])
+    x = _rand(g, rows, d_in, dtype=DT[dtype])
+    inf = float("inf")
+    x[0, d_in - 1], x[rows // 2, 3], x[rows - 1, 0] = inf, float("nan"), -inf
+    for off, slots in (([0, rows], [1]), (_off([1] * rows), [t % 2 for t in range(rows)])):
+        want, err = net_ref.proj(x, w, None, ad, off, slots)
+        got = layer(x.cuda(), _dev(off), _dev(slots))
+        _close(got, want, err, DT[dtype], "finite outputs")
+        got = got.double().cpu()
+        assert torch.isinf(want).sum() > d_out // 2
+        assert torch.equal(torch.isnan(got), torch.isnan(want)), "NaN"
+        assert torch.equal(got[torch.isinf(want)], want[torch.isinf(want)]), "infinities"
