@@ -23,6 +23,7 @@
 #include "psgpu_net_dev.h"
 #include <cmath>
 #include <cstring>
+#include <mutex>
 #include <new>
 #include <type_traits>
 
@@ -37,6 +38,9 @@ struct psgpu_proj_s {
     int32_t *rank = nullptr;                        // [max_adapters], 0: nothing loaded
     float *scale = nullptr;
     char *raw = nullptr;                            // an adapter as it comes, before it is laid out
+    // held by a load from before it waits for the device until its adapter is whole (`raw` is one for all slots), and by a run while it
+    // queues its launches: those in front of a load have ended before it begins, those behind it find it done
+    std::mutex busy;
 };
 
 constexpr int kProjNoRow = -2;                      // rows of no utterance: left as they are
@@ -739,6 +743,7 @@ extern "C" int psgpu_proj_set_adapter(psgpu_proj_t *p, int32_t slot, int32_t ran
     PSGPU_REQUIRE(rank == 0 || std::isfinite(scale), "psgpu_proj_set_adapter: scale %g", (double)scale);
     PSGPU_REQUIRE(psgpu_get_device() == p->device, "psgpu_proj_set_adapter: the projection lives on device %d, the current one is %d", p->device, psgpu_get_device());
     const size_t es = net_dtype_size(p->dtype), raw_a = (size_t)rank * p->d_in * es, at_b = (raw_a + 15) / 16 * 16;
+    std::lock_guard<std::mutex> lock(p->busy);
     PSGPU_HIP(hipDeviceSynchronize());              // calls that read the slot have ended; later ones see it whole
     proj_load_kernel<<<1, 1>>>(p->rank, p->scale, slot, 0, 0.0f);                   // (a copy that fails leaves the slot empty)
     PSGPU_HIP(hipGetLastError());
@@ -875,6 +880,7 @@ extern "C" int psgpu_proj_run_dev(psgpu_proj_t *p, const void *x_dev, int64_t x_
     PSGPU_REQUIRE(device == p->device, "psgpu_proj_run_dev: the projection lives on device %d, the current one is %d", p->device, device);
     const hipStream_t st = (hipStream_t)stream;
     char *work = (char *)work_dev;
+    std::lock_guard<std::mutex> lock(p->busy);
 #define RUN(T, Y) proj_launch<T, Y>(p, x_dev, x_stride, utt_off_dev, adapter_dev, n_utt, total_frames, y_dev, y_stride, work, st)
     if (p->dtype == PSGPU_DT_F32) RUN(float, float);
     else if (p->dtype == PSGPU_DT_F16) { if (y_dtype == PSGPU_DT_F32) RUN(psg_half, float); else RUN(psg_half, psg_half); }

@@ -1,5 +1,7 @@
 """The operators of an acoustic network where numbers end: outputs far from zero, non-finite adapters, the bits that sums are held in,
 adapters loaded while other threads decode.  Bounds are those of tests/net_ref.py unless a test derives its own."""
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -195,3 +197,59 @@ def test_non_finite_inputs_go_through_as_the_formula_says(rows, d_out, rank, dty
         assert torch.isinf(want).sum() > d_out // 2
         assert torch.equal(torch.isnan(got), torch.isnan(want)), "NaN"
         assert torch.equal(got[torch.isinf(want)], want[torch.isinf(want)]), "infinities"
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_adapters_loaded_by_several_threads(dtype):
+    """two threads load their speakers from the host, over and over, while two others decode on streams of their own: every output is that of
+    one whole adapter, and the last loads are what their threads gave"""
+    g = torch.Generator().manual_seed(670)
+    d_in, d_out = 200, 300
+    w = _rand(g, d_out, d_in, dtype=DT[dtype])
+    layer = AdaptedProjection(w, None, 2, 32)
+    x = {n: _rand(g, n, d_in, dtype=DT[dtype]).cuda() for n in (3, 700)}
+    off = {n: _dev([0, n]) for n in x}
+    slot = [_dev([0]), _dev([1])]
+    choices = [[(_rand(g, r, d_in, dtype=DT[dtype]), _rand(g, d_out, r, dtype=DT[dtype]), 0.5) for r in (32, 7)] for _ in range(2)]
+    want = {}
+    for k in range(2):
+        for c, ad in enumerate(choices[k]):
+            layer.set_adapter(k, *ad)
+            for n in x:
+                want[k, c, n] = layer(x[n], off[n], slot[k])
+    torch.cuda.synchronize()
+    wrong, loading = [], [True, True]
+
+    def load(k):
+        try:
+            for i in range(150):
+                layer.set_adapter(k, *choices[k][i % 2])
+        except Exception as e:                              # noqa: BLE001 (a thread's failure is the test's)
+            wrong.append(repr(e))
+        loading[k] = False
+
+    def decode(n):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for i in range(3000):
+                    if not any(loading):
+                        break
+                    k = i & 1
+                    y = layer(x[n], off[n], slot[k])
+                    if not any(torch.equal(y, want[k, c, n]) for c in range(2)):
+                        wrong.append("%d rows, slot %d: neither adapter's result" % (n, k))
+                        break
+            stream.synchronize()
+        except Exception as e:                              # noqa: BLE001
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=load, args=(k,)) for k in range(2)] + [threading.Thread(target=decode, args=(n,)) for n in x]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong
+    for k in range(2):
+        for n in x:
+            assert torch.equal(layer(x[n], off[n], slot[k]), want[k, 1, n])
