@@ -1190,12 +1190,12 @@ int psgpu_hmm_vit_eval(psgpu_hmm_ctx_t *c, psgpu_hmm_rec_t *recs, int32_t n,
 /* y[t] = bias + W x[t] + scale_a B_a (A_a x[t]), a the adapter of row t's utterance: a shared transform (what -lda is for the features,
  * lda.c:139-159) with each speaker's own correction (what -mllr is for one decoder's means).  The object lives on the device that is
  * current at its creation, where its calls must be made.
- *  weight        [d_out][d_in] of `dtype`; bias [d_out] float, or NULL (both in host or in device memory)
+ *  weight        [d_out][d_in] of `dtype`; bias [d_out] float, or NULL (both in host memory or in a device's, which is waited for)
  *  max_adapters  slots for adapters, max_rank (1..PSGPU_PROJ_MAX_RANK) the largest rank one may have
- * psgpu_proj_set_adapter: a [rank][d_in] and b [d_out][rank] of `dtype`, in host or device memory, into a slot (replacing what it holds); rank 0 (a, b NULL)
- * empties it.  It waits for the device, and calls of other threads on the object wait for it, so that no call sees half an adapter; a graph
- * replayed afterwards uses the new one.  What it cannot hold back is a graph's launch, and a capture by another thread does not allow a wait for the
- * device: neither may happen during it.
+ * psgpu_proj_set_adapter: a [rank][d_in] and b [d_out][rank] of `dtype`, in host memory or a device's, into a slot (replacing what it
+ * holds); rank 0 (a, b NULL) empties it.  It waits for the device (and for the weights' own, where that is another), and calls of other
+ * threads on the object wait for it, so that no call sees half an adapter; a graph replayed afterwards uses the new one.  What it cannot
+ * hold back is a graph's launch, and a capture by another thread does not allow a wait for the device: neither may happen during it.
  * psgpu_proj_run_dev: x_dev [total_frames][x_stride], y_dev [total_frames][y_stride] of y_dtype (`dtype` or PSGPU_DT_F32), not
  * overlapping.  utt_off_dev NULL: every row, no adapters (adapter_dev NULL).  adapter_dev [n_utt] slots; any value that names no
  * loaded adapter (-1 by convention) means none.  work_dev: psgpu_proj_work_bytes(p, total_frames) bytes, 16-byte aligned, not needed

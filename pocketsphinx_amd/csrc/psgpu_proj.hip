@@ -676,11 +676,32 @@ static void proj_lay_ab(const psgpu_proj_t *p, int32_t slot, int32_t rank, const
                                                                 (typename proj_b_type<T>::type *)(p->b + slot * p->b_slot));
 }
 
+// where an address lies: the device whose memory it is in, -1: the host
+static int proj_device_of(const void *v)
+{
+    hipPointerAttribute_t at;
+    if (hipPointerGetAttributes(&at, v) != hipSuccess) { (void)hipGetLastError(); return -1; }
+    return at.type == hipMemoryTypeDevice ? at.device : -1;
+}
+
+// what the device of these weights still has to do may be to write them (the current device is waited for anyway)
+static int proj_wait_for(const psgpu_proj_t *p, const void *v)
+{
+    const int device = v ? proj_device_of(v) : -1;
+    if (device < 0 || device == p->device) return PSGPU_OK;
+    proj_on_device on(device);
+    PSGPU_HIP(hipDeviceSynchronize());
+    return PSGPU_OK;
+}
+
 static int proj_fill(psgpu_proj_t *p, const void *weight, const float *bias)
 {
     const size_t es = net_dtype_size(p->dtype), na = (size_t)p->max_adapters;
     const size_t raw_w = (size_t)p->d_out * p->d_in * es, raw_ab = na ? (size_t)p->max_rank * (p->d_in + p->d_out) * es + 32 : 0;
     PSGPU_HIP(hipDeviceSynchronize());              // (weights in device memory are whole)
+    int rc = proj_wait_for(p, weight);
+    if (rc == PSGPU_OK) rc = proj_wait_for(p, bias);
+    if (rc != PSGPU_OK) return rc;
     PSGPU_HIP(hipMalloc((void **)&p->w, (size_t)p->np * p->kp * es));
     PSGPU_HIP(hipMalloc((void **)&p->bias, (size_t)p->np * 4));
     PSGPU_HIP(hipMalloc((void **)&p->raw, raw_w > raw_ab ? raw_w : raw_ab));
@@ -748,11 +769,11 @@ extern "C" int psgpu_proj_set_adapter(psgpu_proj_t *p, int32_t slot, int32_t ran
     proj_load_kernel<<<1, 1>>>(p->rank, p->scale, slot, 0, 0.0f);                   // (a copy that fails leaves the slot empty)
     PSGPU_HIP(hipGetLastError());
     if (rank) {
-        auto here = [&](const void *v) {            // in this device's memory, at an address that its type asks for
-            hipPointerAttribute_t at;
-            if (hipPointerGetAttributes(&at, v) != hipSuccess) { (void)hipGetLastError(); return false; }
-            return at.type == hipMemoryTypeDevice && at.device == p->device && ((uintptr_t)v & (es - 1)) == 0;
-        };
+        int rc = proj_wait_for(p, a);
+        if (rc == PSGPU_OK) rc = proj_wait_for(p, b);
+        if (rc != PSGPU_OK) return rc;
+        // in this device's memory, at an address that its type asks for
+        auto here = [&](const void *v) { return proj_device_of(v) == p->device && ((uintptr_t)v & (es - 1)) == 0; };
         if (!here(a)) {
             PSGPU_HIP(hipMemcpy(p->raw, a, raw_a, hipMemcpyDefault));
             a = p->raw;
