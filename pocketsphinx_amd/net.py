@@ -7,7 +7,7 @@ Tensors are torch's, on the device: rows [frames][width], rows of utterances bac
 bfloat16.  utt_off is an int32 tensor [n_utt + 1] of row offsets; rows of no utterance are left as they are in the output (in an
 output that these functions make themselves they hold nothing defined).  Calls are queued on torch's current stream of the tensors' device and
 can be captured into a graph; workspaces come from torch's allocator, call by call.  They compute forward alone: a tensor that asks for a
-gradient is refused where torch records one."""
+gradient is refused where torch records one, and so is one with a tangent of forward-mode differentiation."""
 import ctypes as C
 
 import numpy as np
@@ -50,6 +50,15 @@ class _On:
             torch.cuda.set_device(self.back)
 
 
+def _no_gradient(t, name):
+    import torch
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError("%s asks for a gradient, and there is none here (torch.no_grad())" % name)
+    forward = torch.autograd.forward_ad
+    if getattr(forward, "_current_level", 0) >= 0 and forward.unpack_dual(t).tangent is not None:       # (outside of a level nothing has one)
+        raise ValueError("%s has a tangent, and there is no forward-mode gradient here (detach())" % name)
+
+
 def _rows(t, name, width=None, dtype=None, device=None, rows=None):
     """checks a 2-d device tensor of rows; returns its row stride in elements"""
     import torch
@@ -59,8 +68,7 @@ def _rows(t, name, width=None, dtype=None, device=None, rows=None):
         raise ValueError("%s is on %s, not on %s" % (name, t.device, device if device is not None else "a GPU"))
     if dtype is not None and t.dtype != dtype:
         raise ValueError("%s has type %s, not %s" % (name, t.dtype, dtype))
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError("%s asks for a gradient, and there is none here (torch.no_grad())" % name)
+    _no_gradient(t, name)
     (n, w), (stride, step) = t.shape, t.stride()
     if width is not None and w != width:
         raise ValueError("%s has rows of %d, not of %d" % (name, w, width))
@@ -81,8 +89,7 @@ def _vector(t, name, n, dtype, device):
     import torch
     if not isinstance(t, torch.Tensor) or t.dim() != 1 or t.dtype != dtype or t.device != device or (n is not None and t.shape[0] != n):
         raise ValueError("%s: a tensor %s of %s on %s is needed" % (name, "[%d]" % n if n is not None else "[n]", dtype, device))
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError("%s asks for a gradient, and there is none here (torch.no_grad())" % name)
+    _no_gradient(t, name)
     return t.contiguous()
 
 

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import net_ref
-from pocketsphinx_amd import AdaptedProjection, senone_scores
+from pocketsphinx_amd import AdaptedProjection, group_norm, senone_scores
 from test_net_gpu import DT, _close, _dev, _layer, _off, _rand
 
 pytestmark = pytest.mark.gpu
@@ -253,3 +253,16 @@ def test_adapters_loaded_by_several_threads(dtype):
     for k in range(2):
         for n in x:
             assert torch.equal(layer(x[n], off[n], slot[k]), want[k, 1, n])
+
+
+def test_tensors_with_a_tangent_are_refused():
+    import torch.autograd.forward_ad as forward
+    x, w = torch.ones(6, 12, device="cuda"), torch.ones(12, device="cuda")
+    layer, off = AdaptedProjection(torch.ones(8, 12)), _dev([0, 6])
+    with forward.dual_level():
+        dx, dw = forward.make_dual(x, torch.ones_like(x)), forward.make_dual(w, torch.ones_like(w))
+        for call in (lambda: group_norm(dx, off, 3), lambda: group_norm(x, off, 3, dw), lambda: group_norm(x, off, 3, None, dw), lambda: senone_scores(dx),
+                     lambda: senone_scores(x, dw), lambda: layer(dx)):
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+        assert torch.equal(layer(dx.detach()), layer(x)) and group_norm(x, off, 3, w).shape == x.shape and senone_scores(x, w).shape == x.shape

@@ -75,3 +75,16 @@ def test_no_cpu_fallback():
     assert _gn() == ENODEV and _ns() == ENODEV
     with pytest.raises(P.PsgpuError):
         P.AdaptedProjection(torch.zeros(4, 4))
+
+
+def test_vectors_with_a_tangent_are_refused():
+    import torch.autograd.forward_ad as forward
+    from pocketsphinx_amd import net
+    v = torch.ones(6)
+    with forward.dual_level():
+        dual = forward.make_dual(v, torch.ones(6))
+        for no_grad in (False, True):               # (which leaves forward mode as it is)
+            with torch.set_grad_enabled(not no_grad), pytest.raises(ValueError, match="tangent"):
+                net._vector(dual, "weight", 6, torch.float32, v.device)
+        assert net._vector(v, "weight", 6, torch.float32, v.device) is v and net._vector(dual.detach(), "weight", 6, torch.float32, v.device).shape == (6,)
+    assert net._vector(v, "weight", 6, torch.float32, v.device) is v
