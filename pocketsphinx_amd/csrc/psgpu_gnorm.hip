@@ -56,12 +56,25 @@ __device__ __forceinline__ float gn_upper_tail(float t)
     return __builtin_amdgcn_exp2f(t * t * -0.72134752044448170f) * (s * p);
 }
 
+// v / (1 + e^-v) through e^-|v| = 2^t, t = -|v| log2 e: for results of 32 bits with what rounding cost t (|v| 2^-24 of the result without it,
+// 20 half-steps at v = -20; nothing that 16 bits show), and with e^v in the numerator below 0, where e^-v could leave float's range.
+// From |v| = 200 on e^-|v| is 0 in any case; an infinity would make a NaN of the difference.
+template <bool SHORT>
+__device__ __forceinline__ float gn_silu(float v)
+{
+    if constexpr (SHORT) return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f));
+    const float a = fminf(fabsf(v), 200.0f), t = a * -1.4426950408889634f;
+    const float r = __builtin_fmaf(a, -1.925963033e-8f, __builtin_fmaf(a, -1.4426950408889634f, -t));
+    const float e0 = __builtin_amdgcn_exp2f(t), e = __builtin_fmaf(e0, r * 0.69314718055994531f, e0);
+    return (v < 0.0f ? v * e : v) * __builtin_amdgcn_rcpf(1.0f + e);
+}
+
 template <int ACT, bool SHORT>
 __device__ __forceinline__ float gn_act(float v)
 {
     switch (ACT) {
     case PSGPU_ACT_RELU: return v < 0.0f ? 0.0f : v;                              // (a NaN stays one)
-    case PSGPU_ACT_SILU: return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f));
+    case PSGPU_ACT_SILU: return gn_silu<SHORT>(v);
     case PSGPU_ACT_GELU: {
         const float q = gn_upper_tail<SHORT>(fabsf(v));
         return v * (v < 0.0f ? q : 1.0f - q);

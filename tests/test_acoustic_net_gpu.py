@@ -266,3 +266,20 @@ def test_tensors_with_a_tangent_are_refused():
             with pytest.raises(ValueError, match="tangent"):
                 call()
         assert torch.equal(layer(dx.detach()), layer(x)) and group_norm(x, off, 3, w).shape == x.shape and senone_scores(x, w).shape == x.shape
+
+
+def test_silu_keeps_32_bits_below_zero():
+    """relative to the value, not to its argument: exp2 and the reciprocal are good to 2 U each, four more roundings to U each (the argument's
+    own is taken back).  A gain of 0 leaves the offset as the argument, exactly; infinite offsets, and beyond the range of exp"""
+    v = torch.cat([torch.linspace(-80, 40, 4096), torch.tensor([0.0, 1e-30, -1e-30, 250.0, 1e30, float("inf")])])
+    n = v.numel()
+    x = torch.tensor([1.0, -1.0]).repeat(n // 2)[None].cuda()
+    y = group_norm(x, _dev([0, 1]), 1, torch.zeros(n, device="cuda"), v.cuda(), act="silu")[0].double().cpu()
+    want = v.double() * torch.sigmoid(v.double())
+    assert y[-1] == float("inf")
+    assert ((y[:-1] - want[:-1]).abs() <= 8 * net_ref.U * want[:-1].abs()).all()
+    far = torch.tensor([-120.0, -1e4, -3e38, -95.0])
+    y = group_norm(x[:, :4].contiguous(), _dev([0, 1]), 1, torch.zeros(4, device="cuda"), far.cuda(), act="silu")[0].cpu()
+    assert (y.abs() <= 95 * np.exp(-95.0)).all() and not torch.isnan(y).any()
+    nan = torch.tensor([float("nan"), -float("inf")], device="cuda")
+    assert torch.isnan(group_norm(x[:, :2].contiguous(), _dev([0, 1]), 1, torch.zeros(2, device="cuda"), nan, act="silu")).all()
