@@ -101,6 +101,14 @@ def _offsets(utt_off, device):
     return utt_off, int(utt_off.shape[0]) - 1
 
 
+def _int32(v, name):
+    """a whole number that the C calls can take (ctypes cuts off what 32 bits do not hold: 2^32 would be 0)"""
+    n = int(v)
+    if n != v or not -0x80000000 <= n <= 0x7fffffff:
+        raise ValueError("%s: %r is no whole number of 32 bits" % (name, v))
+    return n
+
+
 def _p(t):
     return None if t is None else t.data_ptr()
 
@@ -125,7 +133,7 @@ class AdaptedProjection:
         w = _matrix(weight, "weight [d_out][d_in]")
         self.dtype = w.dtype
         self.d_out, self.d_in = int(w.shape[0]), int(w.shape[1])
-        self.max_adapters, self.max_rank = int(max_adapters), int(max_rank)
+        self.max_adapters, self.max_rank = _int32(max_adapters, "max_adapters"), _int32(max_rank, "max_rank")
         b = None
         if bias is not None:
             b = (bias if torch.is_tensor(bias) else torch.from_numpy(np.ascontiguousarray(bias))).detach().float().contiguous()
@@ -149,7 +157,7 @@ class AdaptedProjection:
             if rank < 1 or tuple(a.shape) != (rank, self.d_in) or tuple(b.shape) != (self.d_out, rank):
                 raise ValueError("a [rank][%d] and b [%d][rank] are needed" % (self.d_in, self.d_out))
         with torch.cuda.device(self.device):
-            capi.check(capi.lib().psgpu_proj_set_adapter(self.h, int(slot), rank, _p(a), _p(b), float(scale)), "psgpu_proj_set_adapter")
+            capi.check(capi.lib().psgpu_proj_set_adapter(self.h, _int32(slot, "slot"), rank, _p(a), _p(b), float(scale)), "psgpu_proj_set_adapter")
 
     def __call__(self, x, utt_off=None, adapter=None, out=None, out_dtype=None):
         """x [frames][d_in] of the layer's type -> [frames][d_out] of it or of out_dtype = torch.float32.  utt_off: int32 [n_utt + 1];
@@ -198,6 +206,7 @@ def group_norm(x, utt_off, n_groups, weight=None, bias=None, eps=1e-5, act="none
         raise ValueError("x has type %s" % x.dtype)
     if act not in ACTIVATIONS:
         raise ValueError("act: one of %s" % ", ".join(ACTIVATIONS))
+    n_groups = _int32(n_groups, "n_groups")
     (rows, chan), dev = x.shape, x.device
     utt_off, n_utt = _offsets(utt_off, dev)
     weight = None if weight is None else _vector(weight, "weight", chan, torch.float32, dev)
@@ -207,9 +216,9 @@ def group_norm(x, utt_off, n_groups, weight=None, bias=None, eps=1e-5, act="none
         if out is None:
             out = x.new_empty((rows, chan))
         ys = _rows(out, "out", chan, x.dtype, dev, rows)
-        need = int(L.psgpu_group_norm_work_bytes(n_utt, rows, int(n_groups)))
+        need = int(L.psgpu_group_norm_work_bytes(n_utt, rows, n_groups))
         work = x.new_empty(need, dtype=torch.uint8) if need else None
-        capi.check(L.psgpu_group_norm_dev(_dtypes()[x.dtype], _p(x), xs, _p(utt_off), n_utt, rows, chan, int(n_groups), _p(weight), _p(bias),
+        capi.check(L.psgpu_group_norm_dev(_dtypes()[x.dtype], _p(x), xs, _p(utt_off), n_utt, rows, chan, n_groups, _p(weight), _p(bias),
                                           float(eps), ACTIVATIONS[act], _p(out), ys, _p(work), need, stream), "psgpu_group_norm_dev")
     return out
 

@@ -283,3 +283,15 @@ def test_silu_keeps_32_bits_below_zero():
     assert (y.abs() <= 95 * np.exp(-95.0)).all() and not torch.isnan(y).any()
     nan = torch.tensor([float("nan"), -float("inf")], device="cuda")
     assert torch.isnan(group_norm(x[:, :2].contiguous(), _dev([0, 1]), 1, torch.zeros(2, device="cuda"), nan, act="silu")).all()
+
+
+def test_numbers_beyond_32_bits_are_refused():
+    layer = AdaptedProjection(torch.zeros(8, 12), None, 2, 4)
+    layer.set_adapter(0, torch.ones(2, 12), torch.ones(8, 2))
+    x, off = torch.ones(6, 12, device="cuda"), _dev([0, 6])
+    with pytest.raises(ValueError):
+        layer.set_adapter(1 << 32, None, None)
+    assert (layer(x, off, _dev([0])) == 24.0).all()
+    for n in ((1 << 32) + 3, 1 << 31):
+        with pytest.raises(ValueError):
+            group_norm(x, off, n)

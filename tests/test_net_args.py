@@ -88,3 +88,15 @@ def test_vectors_with_a_tangent_are_refused():
                 net._vector(dual, "weight", 6, torch.float32, v.device)
         assert net._vector(v, "weight", 6, torch.float32, v.device) is v and net._vector(dual.detach(), "weight", 6, torch.float32, v.device).shape == (6,)
     assert net._vector(v, "weight", 6, torch.float32, v.device) is v
+
+
+@pytest.mark.parametrize("v", [1 << 32, (1 << 32) + 3, 1 << 31, -(1 << 31) - 1, 3.5, "3", float("nan")])
+def test_whole_numbers_of_32_bits(v):
+    """what C would cut to another number: a slot of 2^32 is not slot 0"""
+    from pocketsphinx_amd import net
+    with pytest.raises(ValueError):
+        net._int32(v, "slot")
+    for kw in (dict(max_adapters=v), dict(max_adapters=1, max_rank=v)):
+        with pytest.raises(ValueError):
+            P.AdaptedProjection(torch.zeros(4, 4), **kw)
+    assert net._int32(np.int64(7), "slot") == 7 and net._int32(32.0, "slot") == 32 and net._int32(-(1 << 31), "slot") == -(1 << 31) and net._int32((1 << 31) - 1, "slot") == (1 << 31) - 1
