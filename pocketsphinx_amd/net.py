@@ -54,8 +54,7 @@ def _no_gradient(t, name):
     import torch
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError("%s asks for a gradient, and there is none here (torch.no_grad())" % name)
-    forward = torch.autograd.forward_ad
-    if getattr(forward, "_current_level", 0) >= 0 and forward.unpack_dual(t).tangent is not None:       # (outside of a level nothing has one)
+    if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
         raise ValueError("%s has a tangent, and there is no forward-mode gradient here (detach())" % name)
 
 
@@ -68,7 +67,8 @@ def _rows(t, name, width=None, dtype=None, device=None, rows=None):
         raise ValueError("%s is on %s, not on %s" % (name, t.device, device if device is not None else "a GPU"))
     if dtype is not None and t.dtype != dtype:
         raise ValueError("%s has type %s, not %s" % (name, t.dtype, dtype))
-    _no_gradient(t, name)
+    if t.requires_grad or torch.autograd.forward_ad._current_level >= 0:       # (outside of a level nothing has a tangent)
+        _no_gradient(t, name)
     (n, w), (stride, step) = t.shape, t.stride()
     if width is not None and w != width:
         raise ValueError("%s has rows of %d, not of %d" % (name, w, width))
@@ -89,20 +89,23 @@ def _vector(t, name, n, dtype, device):
     import torch
     if not isinstance(t, torch.Tensor) or t.dim() != 1 or t.dtype != dtype or t.device != device or (n is not None and t.shape[0] != n):
         raise ValueError("%s: a tensor %s of %s on %s is needed" % (name, "[%d]" % n if n is not None else "[n]", dtype, device))
-    _no_gradient(t, name)
-    return t.contiguous()
+    if dtype is not torch.int32 and (t.requires_grad or torch.autograd.forward_ad._current_level >= 0):
+        _no_gradient(t, name)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _offsets(utt_off, device):
     import torch
     utt_off = _vector(utt_off, "utt_off", None, torch.int32, device)
-    if utt_off.shape[0] < 1:
+    if not utt_off.shape[0]:
         raise ValueError("utt_off: at least one offset")
-    return utt_off, int(utt_off.shape[0]) - 1
+    return utt_off, utt_off.shape[0] - 1
 
 
 def _int32(v, name):
     """a whole number that the C calls can take (ctypes cuts off what 32 bits do not hold: 2^32 would be 0)"""
+    if type(v) is int and -0x80000000 <= v <= 0x7fffffff:
+        return v
     n = int(v)
     if n != v or not -0x80000000 <= n <= 0x7fffffff:
         raise ValueError("%s: %r is no whole number of 32 bits" % (name, v))
