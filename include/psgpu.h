@@ -1197,9 +1197,10 @@ int psgpu_hmm_vit_eval(psgpu_hmm_ctx_t *c, psgpu_hmm_rec_t *recs, int32_t n,
  * threads on the object wait for it, so that no call sees half an adapter; a graph replayed afterwards uses the new one.  What it cannot
  * hold back is a graph's launch, and a capture by another thread does not allow a wait for the device: neither may happen during it.
  * psgpu_proj_run_dev: x_dev [total_frames][x_stride], y_dev [total_frames][y_stride] of y_dtype (`dtype` or PSGPU_DT_F32), not
- * overlapping.  utt_off_dev NULL: every row, no adapters (adapter_dev NULL).  adapter_dev [n_utt] slots; any value that names no
- * loaded adapter (-1 by convention) means none.  work_dev: psgpu_proj_work_bytes(p, total_frames) bytes, 16-byte aligned, not needed
- * without utt_off_dev. */
+ * overlapping from first row to last (columns of one buffer do).  utt_off_dev NULL: every row, no adapters (adapter_dev NULL).
+ * adapter_dev [n_utt] slots; any value that names no loaded adapter (-1 by convention) means none.  work_dev: psgpu_proj_work_bytes(p,
+ * total_frames) bytes, 16-byte aligned, not needed without utt_off_dev.  A row of x with an infinity or a NaN gives what the formula
+ * gives, in that row alone; an adapter with one gives outputs that are not finite (either kind), in its own utterances' rows alone. */
 typedef struct psgpu_proj_s psgpu_proj_t;
 int psgpu_proj_create(psgpu_proj_t **out, int32_t dtype, int32_t d_in, int32_t d_out, const void *weight, const float *bias,
                       int32_t max_adapters, int32_t max_rank);

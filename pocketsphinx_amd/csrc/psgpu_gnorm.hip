@@ -4,7 +4,7 @@
 //   y[t, c]  = act((x[t, c] - m) / sqrt(v + eps) * weight[c] + bias[c])
 //
 // What cmn() with -varnorm is for cepstra (reference src/feat/cmn.c:166-233), per group of channels and with a learned scale.
-// Sums run in 64 bits: sum x^2 - n m^2 then keeps its digits for groups whose mean is far above their spread.
+// Sums run in 64 bits: sum x^2 - n m^2 is off by a few (m^2 / v) 2^-53 of it, which 32 bits do not show up to a mean of 10^4 spreads.
 //
 // Every kernel works on a slice of whole neighbouring groups of some rows: a work-item has one chunk of 16 bytes of the slice's
 // channels and every nrl-th row, so a wavefront reads rows in one piece at any alignment.  Memory bounds them all.
@@ -26,9 +26,10 @@ struct gn_args {
 
 struct gn_stat { float mhi, mlo, rstd; };               // the mean in two parts
 
-// 1 - (the normal distribution's integral up to t >= 0) = exp(-t^2 / 2) s P(s), s = 1 / (1 + a t): P a least-maximum fit of its
-// relative error over 0 <= t <= 14, beyond which the result is 0 in 32 bits: 1.6e-8 with a = 0.21 and degree 8, for results of 16 bits
-// 8.7e-7 with a = 0.36 and degree 6.  erff() took three times the instructions and bound the kernel.
+// 1 - (the normal distribution's integral up to t >= 0) = exp(-t^2 / 2) s P(s), s = 1 / (1 + a t), the form of Hastings (Approximations for
+// Digital Computers, 1955); P an own fit, whose relative error swings between equal extremes over 0 <= t <= 14, beyond which the result is 0
+// in 32 bits: 1.6e-8 with a = 0.21 and degree 8; for results of 16 bits 8.7e-7 with a = 0.36 and degree 6, a 500th of float16's
+// half-step.  erff() took three times the instructions and bound the kernel.
 template <bool SHORT>
 __device__ __forceinline__ float gn_upper_tail(float t)
 {
@@ -284,7 +285,7 @@ void gnorm_held_kernel(gn_args a)
 // results leave the next one's rows come into the registers that they free.  (Without that a compute unit's two workgroups load,
 // compute and store in step: 634 us for 384 k rows of 1024 in 32 groups.)  Neighbouring groups, which share lines of memory, run on
 // one die (workgroups are dealt to the 8 dies in turn; 577 -> 534 us).  384 k rows of 1024 in 32 groups with GELU: 505 us, 3.1 TB/s; 280
-// us of it are vector instructions, 28 a value.
+// us of it are vector instructions, 28 a value, which the memory's time comes on top of: all 16 wavefronts are in one phase.
 template <typename T, int NT, int NCH, int ACT>
 __global__ __launch_bounds__(NT, 4)
 void gnorm_stream_kernel(gn_args a)
@@ -376,7 +377,9 @@ void gnorm_stream_kernel(gn_args a)
     }
 }
 
-// ---- tiles of rows, in two passes: 102 k rows of 429 floats in 47 + 95 us, 3.7 TB/s ----------------------------------------------------------------------------------------------------
+// ---- tiles of rows, in two passes: 102 k rows of 429 floats in 47 + 94 us, 3.7 TB/s ------------------------------------------------------
+// Every tile of the second pass sums all of its utterance's tiles anew, which is nothing for 30 s of audio (188 tiles: 24 us in all for one
+// utterance) but grows with the square of its length: 65536 frames of 1024 in bfloat16 take 964 us, where a copy takes 38.
 // Rows row .. tile_end - 1 begin in which utterance, and how far it reaches; false: no more utterances in the tile.  Partial sums lie
 // at tile + utterance: along the rows one of the two grows from piece to piece, so every piece has a place of its own.
 __device__ __forceinline__ bool gn_next(const gn_args &a, int &row, int tile_end, int &u, int &end)
@@ -471,7 +474,9 @@ void gnorm_apply_kernel(gn_args a)
 }
 
 // ---- which way ---------------------------------------------------------------------------------------------------------------------
-constexpr int kGnTiles = 4096;                          // (102 k rows of 429 floats: 142 us, with 2048 149)
+// At most so many tiles.  102 k rows of 429 in 11 groups, 1024 / 2048 / 4096 / 8192 of them: float32 145 / 151 / 142 / 149 us, bfloat16 109 / 125 /
+// 143 / 188; 12800 rows: the same within 1 %.
+constexpr int kGnTiles = 4096;
 
 // rows of a tile: about kGnTiles tiles, of 16 rows or more
 static inline int32_t gn_tile_rows(int32_t total) { const int32_t r = (int32_t)(((int64_t)total + kGnTiles - 1) / kGnTiles); return r < 16 ? 16 : (r + 15) / 16 * 16; }
@@ -502,7 +507,12 @@ static void gn_run(gn_args a, hipStream_t st)
     auto chunks = [&](int64_t g) { return mean_len * ((g * a.per + E - 1) / E); };      // of an utterance's slice of g groups
     auto slices = [&](int64_t g) { return (a.n_groups + g - 1) / g; };
     // One launch where an utterance's group fits a workgroup's registers on average and there are enough of them: 256 work-items hold
-    // 8 chunks each, 1024 hold 12.
+    // 8 chunks each, 1024 hold 12.  1024 channels in 32 groups of bfloat16, held / stream / tiles, us (a replayed graph, 15 us of which are
+    // the replay): 1 utterance of 64 frames 16.4 / - / 17.1, of 256 16.1 / - / 17.4; 4 of 500 17.8 / 18.7 / 23.6, 8 of 500 18.5 / 18.3 / 24.2, 16 of
+    // 500 19.4 / 25.2 / 31.0; 64 of 256 23.2 / 69.5 / 33.6, of 512 41.6 / 73.3 / 53.0, of 1024 90.0 / 89.1 / 94.4.  Stream / tiles: 4 of 2000
+    // 24.2 / 27.9, 16 of 2000 39.9 / 61.5, 32 of 2000 67 / 105, 64 of 2048 187 / 180, of 4096 356 / 322; float32 64 of 1024 143 / 168, of 2048 271 / 308.
+    // The mean length decides, for the offsets are on the device: one long utterance among many short ones is one workgroup's a group, row
+    // by row behind its registers (30 s among 511 single frames: 1330 us).
     const bool near_rows = a.xs < 1 << 16 && a.ys < 1 << 16;       // 1024 x 12 rows of them lie within 2^32 bytes
     if (near_rows && chunks(1) <= 256 * 8 && ((int64_t)a.total * a.n_chan <= 1 << 17 || (int64_t)a.n_utt * a.n_groups >= 256)) {
         while (gs > 1 && (chunks(gs) > 256 * 8 || a.n_utt * slices(gs) < 512)) gs = (gs + 1) / 2;

@@ -78,7 +78,7 @@ __device__ __forceinline__ unsigned long long scr_key(double v)
 __device__ __forceinline__ double scr_value(unsigned long long k) { return __longlong_as_double((long long)(k >> 63 ? k ^ 1ull << 63 : ~k)); }
 
 // A row a workgroup, NCH chunks of 16 bytes a work-item, in registers, the next row on its way; the priors are fetched once for all of
-// a workgroup's rows.  96 k rows of 5126 in bfloat16: 536 us, 3.7 TB/s; vector instructions, 29 a value, are 360 us of it.
+// a workgroup's rows.  96 k rows of 5126 in bfloat16: 533 us, 3.7 TB/s; vector instructions, 29 a value, are 360 us of it.
 //
 // l in 32 bits, lf = fl(z - prior), keeps the order: the best l is among those whose lf is the greatest, and only those are taken in 64
 // bits.  A score's q = (top - l) unit + 1/2 in 32 bits is off by at most c + 6 q 2^-23, c = (2 |top| unit + 4) 2^-23: the three
@@ -256,8 +256,10 @@ static void scr_run(const void *z, int64_t zs, int32_t rows, int32_t n_sen, cons
     constexpr int E = 16 / sizeof(T);
     const int plain = unit >= 1e-6 && unit <= 1e6;
     const int64_t chunks = ((int64_t)n_sen + E - 1) / E;
-    // Workgroups that run at once (4 a compute unit), or twice as many where a row more or less in some does not count (5120 rows of
-    // 5126: 41.7 against 45.8 us; 96 k rows: 592 against 573); few rows: all of a compute unit's wavefronts on each
+    // Workgroups that run at once (4 a compute unit), or twice as many where a row more or less in some does not count.  Rows of 5126 in
+    // bfloat16, 1024 / 2048 workgroups, us: 4096 rows 38.7 / 43.5, 16384 rows 109 / 111, 32768 rows 199 / 200, 96 k rows 542 / 535; float32: 58.0 / 62.7,
+    // 213 / 217, 413 / 416, 1193 / 1197.  Few rows: all of a compute unit's wavefronts on each.  256 / 1024 work-items a row: 512 rows 16.3 / 17.6, 1024
+    // rows 21.3 / 27.5, 2048 rows 27.7 / 37.6; float32 16.9 / 18.9, 23.8 / 23.9, 35.3 / 35.4; 256 rows and fewer the same.
     const int32_t most = rows < 16384 ? 1024 : 2048;
 #define ROWS(NT, NCH) netscr_row_kernel<T, NT, NCH><<<(uint32_t)(rows < most ? rows : most), NT, 0, st>>>((const T *)z, zs, rows, n_sen, prior, unit, plain, out, os, best)
     if (n_sen < E) netscr_long_kernel<T><<<(uint32_t)rows, kScrThreads, 0, st>>>((const T *)z, zs, n_sen, prior, unit, out, os, best);

@@ -166,8 +166,7 @@ __device__ __forceinline__ void proj_store_h(net_f32x4 v, float scale, char *h, 
 }
 
 // Many rows: MR 16 a wavefront, all of an adapter's ranks at once, x once from memory (that is what bounds it: 384 k rows of 1024 in
-// bfloat16, rank 32: 205 us, 3.8 TB/s), A from the caches (as
-// many bytes as x with 32 rows and 32 ranks: 64 rows where that leaves enough wavefronts).
+// bfloat16, rank 32: 207 us, 4.1 TB/s with h), A from the caches (as many bytes as x with 32 rows and 32 ranks).
 template <typename T, int RF, int MR>
 __global__ __launch_bounds__(256)
 void proj_shrink_kernel(const T *__restrict__ x, int64_t x_stride, int32_t total, int32_t d_in, int32_t chunks, const char *__restrict__ a, size_t a_slot,
@@ -305,9 +304,10 @@ __device__ __forceinline__ void proj_expand(net_f32x4 (&acc)[4], bool mine, cons
 // A tile of BM = WM MF 16 frames x BN = WN 64 outputs a workgroup; a wavefront MF 16 x 64.  A ring of three stages in LDS of 64 bytes
 // of the reduced axis: while one is multiplied the next is there or nearly and the one behind it is on its way.  x lies in rows of 64
 // bytes whose 16-byte pieces are exchanged by the row (piece p of row r at p ^ (r / 2 & 3)), so that 8 lanes meet no bank twice; W
-// lies as in memory.  131072 rows of 1024 to 1024 in bfloat16: with 256 x 256 a workgroup (8 wavefronts, one a compute unit) 335 us, 822
-// TFLOP/s; with 256 x 128 (two a compute unit, whose first loads and last stores pass under the other's products) 360 us: LDS
-// bounds both, for 32 matrix instructions of a wavefront 12 KB are read and 4 KB, there 6 KB, written.
+// lies as in memory.  131072 rows of 1024 to 1024 in bfloat16: with 256 x 256 a workgroup (8 wavefronts, one a compute unit) 323 to 336 us,
+// 820 to 850 TFLOP/s; 256 x 128 (two a compute unit, whose first loads and last stores pass under the other's products) was 7 % slower.  A stage
+// is a barrier, 12 KB of reads and 32 matrix instructions a wavefront one behind the other, all wavefronts in step: the matrix units are
+// 48 % busy, LDS by its bytes (12 KB read, 4 KB written at 128 a cycle) about as much, and neither is full.
 // DMA: x goes to LDS without a register, 16 bytes a lane where it is aligned to them, else 4 bytes (rows of 429 floats),
 // or 0: through registers.  A last stage that d_in does not fill goes through registers.
 // Where all of a tile's frames have one adapter its h and B are more stages of the same ring (h's parts against B's); else every
@@ -811,7 +811,12 @@ static void proj_shrink(const psgpu_proj_t *p, const void *x, int64_t xs, const 
 {
     const int32_t chunks = p->kp / proj_geo<T>::KC;
     const char *a = adapter ? p->a : nullptr;
-    // few rows: one a workgroup up to 2048 of them, so that all run at once
+    // Few rows: 1, 4 or 16 a workgroup.  With the product of 64 outputs behind it, 1024 inputs, rank 16, us:
+    //   bfloat16   1024 rows 17.4 / 16.5 / 18.6   2048 rows 19.8 / 17.1 / 18.7   8192 rows 4: 25.4, 16: 22.5, many: 45.1
+    //   float32    1024 rows 26.2 / 22.6 / 27.6   2048 rows 39.1 / 30.9 / 27.6   8192 rows 4: 44.3, 16: 45.7, many: 89.5
+    // (one a workgroup pays below 1024 rows alone).  Few against many rows: 16384 rows 34.4 / 51.4 and 63.9 / 105.3, 32768 rows 46.3 / 60.1 and 117
+    // / 151.  32 against 64 rows a wavefront: 131072 rows of bfloat16 129 / 133 with ranks 16 and 32, 186 / 156 with rank 64; of float32 428 /
+    // 428, 464 / 450, 513 / 501.
     const bool few = total <= 16384;
     const int32_t tile = total <= 2048 ? 1 : total <= 8192 ? 4 : 16;
     const bool wide = total >= 131072;
@@ -845,6 +850,12 @@ static void proj_launch(const psgpu_proj_t *p, const void *x, int64_t xs, const 
     const char *b = adapter ? p->b : nullptr;
     const size_t b_part = p->b_slot / proj_b_type<T>::parts;
     const uintptr_t at = (uintptr_t)x | (uintptr_t)(xs * sizeof(T));
+    // Tiles of 128 x 128 from 256 of them on (fewer leave compute units idle).  Few rows against tiles, 1024 to 1024, rank 16, us:
+    //   bfloat16   512 rows 19.7 / 28.1   1024 rows 25.5 / 28.8   2048 rows 40.1 / 32.0   4000 rows 60.1 / 32.3   8000 rows 106 / 42
+    //   float32    512 rows 29.8 / 86.5   1024 rows 51.2 / 92.8   2048 rows 82.7 / 99.3   4000 rows 130 / 97      8000 rows 239 / 162
+    // (at the rule, 4096 rows, tiles are ahead already: in bfloat16 from 128 of them on).  Tiles of 256 x 256 from 512 of them on, 128 / 256 us in
+    // bfloat16: 8192 rows 42.0 / 55.1   16384 rows 65.7 / 62.7   32768 rows 122 / 120   65536 rows 208 / 208; not for outputs that leave much of
+    // them empty: 65536 rows to 1040 244 / 261, to 1100 244 / 265, to 2100 412 / 433, to 1280 267 / 268.
     const bool near_rows = xs < ((int64_t)1 << 30) / 256 / (int64_t)sizeof(T);      // (a tile's rows at 32-bit offsets)
     const int dma = !near_rows ? 0 : (at & 15) == 0 ? 16 : (at & 3) == 0 ? 4 : 0;
 #define TILE(D, WM, WN, MF) do { \
@@ -857,10 +868,10 @@ static void proj_launch(const psgpu_proj_t *p, const void *x, int64_t xs, const 
         if (own_h) {
             const dim3 grid((uint32_t)((p->d_out + 63) / 64 * 4), 1);
             proj_few_kernel<T, Y, 4, 1, 1, true><<<grid, 256, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, p->w, p->bias, p->d_out, b, p->b_slot, b_part, p->rp, p->rank, slots, h, (Y *)y, ys, FEW_REST);
-        } else if (total <= 16) {
+        } else if (total <= 16) {       // 16 against 64 outputs a workgroup, 16 rows: 16.5 / 17.4 us, float32 18.7 / 22.1; 64 rows: 19.8 / 19.2, 18.8 / 22.5
             const dim3 grid((uint32_t)((p->d_out + 63) / 64 * 4), 1);
             proj_few_kernel<T, Y, 4, 1, 1, false><<<grid, 256, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, p->w, p->bias, p->d_out, b, p->b_slot, b_part, p->rp, p->rank, slots, h, (Y *)y, ys, FEW_REST);
-        } else if ((int64_t)((p->d_out + 63) / 64) * ((total + 31) / 32) < 512) {      // 512 rows to 1024: 19.5 against 20.8 us
+        } else if ((int64_t)((p->d_out + 63) / 64) * ((total + 31) / 32) < 512) {      // 16 against 32 frames, 512 rows: 20.0 / 20.6 us; 1024 rows: 26.8 / 25.3; 2048 rows: 45.0 / 39.6
             const dim3 grid((uint32_t)((p->d_out + 63) / 64), (uint32_t)((total + 15) / 16));
             proj_few_kernel<T, Y, 4, 1, 4, false><<<grid, 256, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, p->w, p->bias, p->d_out, b, p->b_slot, b_part, p->rp, p->rank, slots, h, (Y *)y, ys, FEW_REST);
         } else {
