@@ -17,7 +17,8 @@
 // The adapters' h is kept in 32 bits, for the half types as three bfloat16 parts of 8 bits each, cut, not rounded, so that their sum is h
 // exactly.  They go through the matrix instructions as more pieces of the reduced axis, against B in bfloat16: float16's B is two
 // parts (exact); the product of the smallest two, 2^-25 of the term, is left out.  In float16 itself h could overflow.  (Two parts
-// were 2^-18 of h, an adapter's term in 32 bits off by 1.3e-6 of its size, 10 times what its sums are.  The third costs 22 of 1058 us for
+// were 2^-18 of h; an adapter's term of rank 32 in 32 bits was off by 2.5e-6 in the mean square, in float16 3.7e-6, and is by 1.2e-7 and
+// 1.5e-7.  The third costs 22 of 1058 us for
 // 384 k rows of 1024 to 1024 in bfloat16 with rank 32, the two more 18 of 660 us for 48 k rows of 1024 to 5126 in float16.)
 // A value that is not finite is a third part alone: against B's second part, often 0, an infinity would be a NaN.
 #include "psgpu_net_dev.h"
@@ -812,9 +813,11 @@ static void proj_shrink(const psgpu_proj_t *p, const void *x, int64_t xs, const 
     const int32_t chunks = p->kp / proj_geo<T>::KC;
     const char *a = adapter ? p->a : nullptr;
     // Few rows: 1, 4 or 16 a workgroup.  With the product of 64 outputs behind it, 1024 inputs, rank 16, us:
+    // in utterances of 100 rows
     //   bfloat16   1024 rows 17.4 / 16.5 / 18.6   2048 rows 19.8 / 17.1 / 18.7   8192 rows 4: 25.4, 16: 22.5, many: 45.1
     //   float32    1024 rows 26.2 / 22.6 / 27.6   2048 rows 39.1 / 30.9 / 27.6   8192 rows 4: 44.3, 16: 45.7, many: 89.5
-    // (one a workgroup pays below 1024 rows alone).  Few against many rows: 16384 rows 34.4 / 51.4 and 63.9 / 105.3, 32768 rows 46.3 / 60.1 and 117
+    // and where every row has another adapter, which a workgroup takes in turn, 1 / 4 / 16: 512 rows 18.0 / 24.4 / 53.6, float32 25.2 / 37.6 / 93.3; 2048
+    // rows 21.7 / 25.4 / 52.7, 38.2 / 47.3 / 93.9.  Few against many rows: 16384 rows 34.4 / 51.4 and 63.9 / 105.3, 32768 rows 46.3 / 60.1 and 117
     // / 151.  32 against 64 rows a wavefront: 131072 rows of bfloat16 129 / 133 with ranks 16 and 32, 186 / 156 with rank 64; of float32 428 /
     // 428, 464 / 450, 513 / 501.
     const bool few = total <= 16384;
@@ -868,10 +871,11 @@ static void proj_launch(const psgpu_proj_t *p, const void *x, int64_t xs, const 
         if (own_h) {
             const dim3 grid((uint32_t)((p->d_out + 63) / 64 * 4), 1);
             proj_few_kernel<T, Y, 4, 1, 1, true><<<grid, 256, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, p->w, p->bias, p->d_out, b, p->b_slot, b_part, p->rp, p->rank, slots, h, (Y *)y, ys, FEW_REST);
-        } else if (total <= 16) {       // 16 against 64 outputs a workgroup, 16 rows: 16.5 / 17.4 us, float32 18.7 / 22.1; 64 rows: 19.8 / 19.2, 18.8 / 22.5
+        } else if (total <= 16) {       // 16 / 64 outputs a workgroup, 16 rows: 16.5 / 17.4 us, float32 18.7 / 22.1; 64 rows: 19.8 / 19.2, 18.8 / 22.5
             const dim3 grid((uint32_t)((p->d_out + 63) / 64 * 4), 1);
             proj_few_kernel<T, Y, 4, 1, 1, false><<<grid, 256, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, p->w, p->bias, p->d_out, b, p->b_slot, b_part, p->rp, p->rank, slots, h, (Y *)y, ys, FEW_REST);
-        } else if ((int64_t)((p->d_out + 63) / 64) * ((total + 31) / 32) < 512) {      // 16 against 32 frames, 512 rows: 20.0 / 20.6 us; 1024 rows: 26.8 / 25.3; 2048 rows: 45.0 / 39.6
+        } else if ((int64_t)((p->d_out + 63) / 64) * ((total + 31) / 32) < 512) {
+            // 16 / 32 frames, 512 rows to 1024: 20.0 / 20.6 us; 1024 rows: 26.8 / 25.3; 2048 rows: 45.0 / 39.6
             const dim3 grid((uint32_t)((p->d_out + 63) / 64), (uint32_t)((total + 15) / 16));
             proj_few_kernel<T, Y, 4, 1, 4, false><<<grid, 256, 0, st>>>((const T *)x, xs, total, p->d_in, chunks, p->w, p->bias, p->d_out, b, p->b_slot, b_part, p->rp, p->rank, slots, h, (Y *)y, ys, FEW_REST);
         } else {
